@@ -317,6 +317,42 @@ int lcc_sample_topk_topp(const void* logits, int ld, int B, int V, uint32_t* see
                          int hist_ld, int32_t* hist_col, float* scores_out, float temperature, int top_k, float top_p,
                          uint64_t seed, uint32_t* rng_ctr, void* stream);
 
+/* ---- KV cache held in 4 bits.  32 channels of one token and KV head share a power of two: value = code * 2^(e - 127), code one of
+ * +-{0 .5 1 1.5 2 3 4 6} in 4 bits, e one byte; e is the smallest with max |x| <= 7 * 2^(e - 127) (2 .. 252), codes are the nearest, ties to the even code;
+ * a group that holds an infinity or a NaN has e = 255 and reads as NaN.  Every value is exact in bf16.  `lay` as for the bf16 cache (head_dim 128,
+ * lmax % 32 == 0); a slot's arena has lcc_kv4_slot_bytes(lay) bytes, 16-byte aligned:
+ *   [layer][K codes [head][lmax][64] | V codes [head][lmax / 32][g 4][i 16][t 4][e 8] | K scales [head][lmax][4] | V scales [head][lmax / 32][g 4][t 4][e 8]]
+ *   K: byte b of a token = channels 2 b (low half), 2 b + 1;  V: byte (g, i, t, e) = position 8 g + e of the block, channels 32 t + i (low half), 32 t + 16 + i.
+ * kv_base: device table of n_slots arenas.  Slots and positions are checked on the device: a row whose slot or position is out of range (-1: a padded
+ * row) appends nothing, reads and attends to nothing (zeros).  (slot, position) pairs of one append are distinct. */
+size_t lcc_kv4_slot_bytes(lcc_kv_layout lay);                                   /* 0: invalid layout */
+/* Between the q|k|v projection and the attention, one pass: [RMS norm of every query and key head: bf16(w * bf16(x * r)), r = 1 / sqrt(mean(x^2) + eps) formed
+ * in 64 bits and rounded once] + M-RoPE (as lcc_rope_kv_append_bf16) + append.  q_norm / k_norm: bf16 [128], NULL: no norm.  Rows: qkv_bf16
+ * [S][(Hq + 2 Hkv) * 128], or fp32 slabs qkv_partial [nsplit <= 8][S][..] (+ bias or NULL).  tok_pos NULL: position kv_len[slot].  n_q_heads 0: append only (q_out
+ * may be NULL).  q_out [S][Hq * 128] of every row, those of no stream too.  First form: the bf16 cache of lcc_rope_kv_append_bf16; second: 4 bits. */
+int lcc_qk_norm_rope_kv_append_bf16(const void* qkv_bf16, const float* qkv_partial, int nsplit, const void* bias, const void* q_norm, const void* k_norm, float eps,
+                                    const void* cos, const void* sin, const int32_t* tok_stream, const int32_t* tok_pos, const int32_t* kv_len,
+                                    void* const* kv_base, int n_slots, lcc_kv_layout lay, int layer, void* q_out, int S, int n_q_heads, void* stream);
+int lcc_qk_norm_rope_kv4_append(const void* qkv_bf16, const float* qkv_partial, int nsplit, const void* bias, const void* q_norm, const void* k_norm, float eps,
+                                const void* cos, const void* sin, const int32_t* tok_stream, const int32_t* tok_pos, const int32_t* kv_len,
+                                void* const* kv_base, int n_slots, lcc_kv_layout lay, int layer, void* q_out, int S, int n_q_heads, void* stream);
+/* keys and values of S (slot, position) pairs out of the 4-bit cache: k_out, v_out bf16 [S][Hkv][128] */
+int lcc_kv4_read(void* const* kv_base, int n_slots, lcc_kv_layout lay, int layer, const int32_t* tok_stream, const int32_t* tok_pos, void* k_out, void* v_out, int S,
+                 void* stream);
+/* attention core as lcc_attn_decode_bf16 over the 4-bit cache: row b sees keys 0 .. kv_len[slots[b]] (-1: none); up to 16 query heads per KV head.
+ * nsplit <= 64 key splits; > 1: scratch ws_o [B * Hq * nsplit * 128], ws_ml [B * Hq * nsplit * 2] floats.  lcc_kv4_decode_splits: the count that suits streams
+ * of n_keys[b] keys (host logic, no GPU) */
+int lcc_kv4_decode_splits(const int32_t* n_keys, int n_streams, int n_kv_heads);
+int lcc_attn_decode_kv4(const void* q, void* out, const int32_t* slots, const int32_t* kv_len, void* const* kv_base, int n_slots, lcc_kv_layout lay, int layer, int B,
+                        int n_q_heads, int nsplit, float* ws_o, float* ws_ml, void* stream);
+/* attention core as lcc_attn_prefill_bf16 over the 4-bit cache: tiles of up to tile_rows (<= 256 / (Hq / Hkv)) consecutive new rows of one stream; a row at
+ * position p sees keys 0 .. p.  Every row of q belongs to exactly one tile.  nsplit <= 32; > 1: scratch ws_o [n_rows * Hq * nsplit * 128], ws_ml [n_rows * Hq *
+ * nsplit * 2].  lcc_kv4_prefill_plan: tile height and split count for streams of n_new[b] rows behind past[b] keys on a device of cu_count compute units (host logic) */
+int lcc_kv4_prefill_plan(const int32_t* n_new, const int32_t* past, int n_streams, int n_q_heads, int n_kv_heads, int cu_count, int32_t* tile_rows, int32_t* nsplit);
+int lcc_attn_prefill_kv4(const void* q, void* out, const int32_t* tile_stream, const int32_t* tile_q0, const int32_t* tile_nq, const int32_t* tile_pos0,
+                         void* const* kv_base, int n_slots, lcc_kv_layout lay, int layer, int n_tiles, int n_q_heads, int tile_rows, int nsplit, int n_rows,
+                         float* ws_o, float* ws_ml, void* stream);
+
 /* ---- layer-list decoders: row operators and latent attention (no reference counterpart).  Channel counts are padded to multiples of 64 with
  * zero weights; the residual stream x is fp32.
  * Dynamic Tanh: y = tanh(alpha x) w + b, alpha one bf16 value, w / b bf16 [dim]: no row statistic. */

@@ -172,6 +172,14 @@ def load():
                                     vp, vp, vp]),
         "lcc_sample_topk_topp": (i32, [vp, i32, i32, i32, vp, i32, vp, f32, i32, i32, f32, i32, i32, i32, vp, vp, vp, i32, vp,
                                        vp, f32, i32, f32, C.c_uint64, vp, vp]),
+        "lcc_kv4_slot_bytes": (sz, [KvLayout]),
+        "lcc_qk_norm_rope_kv_append_bf16": (i32, [vp, vp, i32, vp, vp, vp, f32, vp, vp, vp, vp, vp, vp, i32, KvLayout, i32, vp, i32, i32, vp]),
+        "lcc_qk_norm_rope_kv4_append": (i32, [vp, vp, i32, vp, vp, vp, f32, vp, vp, vp, vp, vp, vp, i32, KvLayout, i32, vp, i32, i32, vp]),
+        "lcc_kv4_read": (i32, [vp, i32, KvLayout, i32, vp, vp, vp, vp, i32, vp]),
+        "lcc_kv4_decode_splits": (i32, [vp, i32, i32]),
+        "lcc_attn_decode_kv4": (i32, [vp, vp, vp, vp, vp, i32, KvLayout, i32, i32, i32, i32, vp, vp, vp]),
+        "lcc_kv4_prefill_plan": (i32, [vp, vp, i32, i32, i32, i32, vp, vp]),
+        "lcc_attn_prefill_kv4": (i32, [vp, vp, vp, vp, vp, vp, vp, i32, KvLayout, i32, i32, i32, i32, i32, i32, vp, vp, vp]),
         "lcc_embed_dyt": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, i32, i32, vp]),
         "lcc_resid_dyt": (i32, [vp, vp, i32, vp, vp, vp, vp, i32, i32, vp]),
         "lcc_logits_cap": (i32, [vp, i32, i32, i32, i32, f32, vp, vp, vp]),

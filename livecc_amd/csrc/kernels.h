@@ -376,4 +376,32 @@ int dgemv_f32(const DgArgs& a, hipStream_t st);
 int dgemv_f32_pair(const DgArgs& a, const DgArgs& b, hipStream_t st);
 int dgemv_swiglu(const DgArgs& a, hipStream_t st);
 
+// ---- KV cache in 4 bits, norm + rotation + append (kv4.hip) ----
+struct Kv4Layout {  // a slot's layer: [K codes | V codes | K scales | V scales], bytes; 136 of them a key and KV head
+  int n_kv_heads, lmax;
+  __host__ __device__ size_t layer_bytes() const { return (size_t)n_kv_heads * lmax * 136; }
+  __host__ __device__ size_t k_codes(int h) const { return (size_t)h * lmax * 64; }
+  __host__ __device__ size_t v_codes(int h) const { return (size_t)(n_kv_heads + h) * lmax * 64; }
+  __host__ __device__ size_t k_scales(int h) const { return (size_t)n_kv_heads * lmax * 128 + (size_t)h * lmax * 4; }
+  __host__ __device__ size_t v_scales(int h) const { return (size_t)n_kv_heads * lmax * 132 + (size_t)h * lmax * 4; }
+};
+struct Kv4Args {
+  void* const* kv_base; int n_slots, n_layers, n_kv_heads, lmax, layer;
+  int check() const { return n_slots < 0 || n_layers < 1 || n_kv_heads < 1 || lmax < 32 || (lmax & 31) || layer < 0 || layer >= n_layers ? LCC_ERR_SHAPE : 0; }
+};
+struct QkNormArgs {
+  const bf16_t* qkv; const float* partial; int nsplit; const bf16_t* bias;      // rows [q heads | k heads | v heads][128]: bf16, or slabs (+ bias)
+  const bf16_t* q_norm; const bf16_t* k_norm; float eps;                        // weights [128]; null: no norm
+  const bf16_t* cos; const bf16_t* sin; const int32_t* tok_stream; const int32_t* tok_pos; const int32_t* kv_len;
+  void* const* kv_base; int n_slots, n_layers, n_kv_heads, lmax, layer; bf16_t* q_out; int rows, n_q_heads;
+};
+int qk_norm_rope_append(const QkNormArgs& a, bool kv4, hipStream_t st);
+int kv4_read(const Kv4Args& a, const int32_t* tok_stream, const int32_t* tok_pos, bf16_t* k, bf16_t* v, int rows, hipStream_t st);
+int kv4_decode_splits(const int32_t* n_keys, int n, int n_kv_heads);
+int attn_decode_kv4(const Kv4Args& a, const bf16_t* q, const int32_t* slots, const int32_t* kv_len, int rows, int n_q_heads, int nsplit, float* ws_o, float* ws_ml,
+                    bf16_t* out, hipStream_t st);
+int kv4_prefill_plan(const int32_t* n_new, const int32_t* past, int n, int n_q_heads, int n_kv_heads, int cus, int* tile_rows, int* nsplit);
+int attn_prefill_kv4(const Kv4Args& a, const bf16_t* q, bf16_t* out, const int32_t* tile_stream, const int32_t* tile_q0, const int32_t* tile_nq, const int32_t* tile_pos0,
+                     int n_tiles, int n_q_heads, int tile_rows, int nsplit, int n_rows, float* ws_o, float* ws_ml, hipStream_t st);
+
 }  // namespace lcc

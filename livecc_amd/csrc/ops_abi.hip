@@ -531,3 +531,75 @@ extern "C" int lcc_latent_attn_decode(const void* q_latent, const int32_t* slots
   if (int r = latent_attn_decode(a, (hipStream_t)stream)) return fail(r, "lcc_latent_attn_decode: invalid arguments (%d)", r);
   OP_RET(latent_merge_uv(a, (const bf16_t*)uv, vdim, gate, (bf16_t*)out, ldo, (hipStream_t)stream), "lcc_latent_attn_decode");
 }
+
+// ---- KV cache in 4 bits (kv4.hip) ----
+static Kv4Args to_kv4(void* const* kv_base, int n_slots, lcc_kv_layout lay, int layer) { return Kv4Args{kv_base, n_slots, lay.n_layers, lay.n_kv_heads, lay.lmax, layer}; }
+static int kv4_lay_ok(lcc_kv_layout lay, const char* name) {
+  if (lay.head_dim != 128) return fail(LCC_ERR_SHAPE, "%s: head_dim must be 128, got %d", name, lay.head_dim);
+  if (lay.n_layers < 1 || lay.n_kv_heads < 1 || lay.lmax < 32 || lay.lmax % 32) return fail(LCC_ERR_SHAPE, "%s: bad cache layout (lmax a multiple of 32)", name);
+  return 0;
+}
+static bool not16(const void* p) { return ((uintptr_t)p & 15) != 0; }
+extern "C" size_t lcc_kv4_slot_bytes(lcc_kv_layout lay) {
+  if (kv4_lay_ok(lay, "lcc_kv4_slot_bytes")) return 0;
+  return (size_t)lay.n_layers * Kv4Layout{lay.n_kv_heads, lay.lmax}.layer_bytes();
+}
+static int qk_norm_entry(bool kv4, const char* name, const void* qkv_bf16, const float* qkv_partial, int nsplit, const void* bias, const void* q_norm, const void* k_norm,
+                         float eps, const void* cos, const void* sin, const int32_t* tok_stream, const int32_t* tok_pos, const int32_t* kv_len, void* const* kv_base,
+                         int n_slots, lcc_kv_layout lay, int layer, void* q_out, int S, int n_q_heads, void* stream) {
+  if ((qkv_bf16 == nullptr) == (qkv_partial == nullptr)) return fail(LCC_ERR_ARG, "%s: exactly one of qkv_bf16 and qkv_partial", name);
+  if (!cos || !sin || !tok_stream || (!tok_pos && !kv_len) || !kv_base || (!q_out && n_q_heads > 0)) return fail(LCC_ERR_ARG, "%s: null pointer", name);
+  if (bias && !qkv_partial) return fail(LCC_ERR_ARG, "%s: a bias goes with qkv_partial", name);
+  if (not16(qkv_bf16) || not16(qkv_partial) || not16(bias) || not16(q_norm) || not16(k_norm) || not16(cos) || not16(sin) || not16(q_out))
+    return fail(LCC_ERR_ALIGN, "%s: pointers must be 16-byte aligned", name);
+  if (int rc = kv4_lay_ok(lay, name)) return rc;
+  QkNormArgs a{(const bf16_t*)qkv_bf16, qkv_partial, nsplit, (const bf16_t*)bias, (const bf16_t*)q_norm, (const bf16_t*)k_norm, eps, (const bf16_t*)cos, (const bf16_t*)sin,
+               tok_stream, tok_pos, kv_len, kv_base, n_slots, lay.n_layers, lay.n_kv_heads, lay.lmax, layer, (bf16_t*)q_out, S, n_q_heads};
+  OP_RET(qk_norm_rope_append(a, kv4, (hipStream_t)stream), name);
+}
+extern "C" int lcc_qk_norm_rope_kv_append_bf16(const void* qkv_bf16, const float* qkv_partial, int nsplit, const void* bias, const void* q_norm, const void* k_norm,
+                                               float eps, const void* cos, const void* sin, const int32_t* tok_stream, const int32_t* tok_pos, const int32_t* kv_len,
+                                               void* const* kv_base, int n_slots, lcc_kv_layout lay, int layer, void* q_out, int S, int n_q_heads, void* stream) {
+  return qk_norm_entry(false, "lcc_qk_norm_rope_kv_append_bf16", qkv_bf16, qkv_partial, nsplit, bias, q_norm, k_norm, eps, cos, sin, tok_stream, tok_pos, kv_len, kv_base,
+                       n_slots, lay, layer, q_out, S, n_q_heads, stream);
+}
+extern "C" int lcc_qk_norm_rope_kv4_append(const void* qkv_bf16, const float* qkv_partial, int nsplit, const void* bias, const void* q_norm, const void* k_norm, float eps,
+                                           const void* cos, const void* sin, const int32_t* tok_stream, const int32_t* tok_pos, const int32_t* kv_len,
+                                           void* const* kv_base, int n_slots, lcc_kv_layout lay, int layer, void* q_out, int S, int n_q_heads, void* stream) {
+  return qk_norm_entry(true, "lcc_qk_norm_rope_kv4_append", qkv_bf16, qkv_partial, nsplit, bias, q_norm, k_norm, eps, cos, sin, tok_stream, tok_pos, kv_len, kv_base,
+                       n_slots, lay, layer, q_out, S, n_q_heads, stream);
+}
+extern "C" int lcc_kv4_read(void* const* kv_base, int n_slots, lcc_kv_layout lay, int layer, const int32_t* tok_stream, const int32_t* tok_pos, void* k_out, void* v_out,
+                            int S, void* stream) {
+  if (!kv_base || !tok_stream || !tok_pos || !k_out || !v_out) return fail(LCC_ERR_ARG, "lcc_kv4_read: null pointer");
+  if (not16(k_out) || not16(v_out)) return fail(LCC_ERR_ALIGN, "lcc_kv4_read: pointers must be 16-byte aligned");
+  if (int rc = kv4_lay_ok(lay, "lcc_kv4_read")) return rc;
+  OP_RET(kv4_read(to_kv4(kv_base, n_slots, lay, layer), tok_stream, tok_pos, (bf16_t*)k_out, (bf16_t*)v_out, S, (hipStream_t)stream), "lcc_kv4_read");
+}
+extern "C" int lcc_kv4_decode_splits(const int32_t* n_keys, int n_streams, int n_kv_heads) {
+  if (n_streams < 1 || !n_keys || n_kv_heads < 1) return fail(LCC_ERR_ARG, "lcc_kv4_decode_splits: bad argument");
+  return kv4_decode_splits(n_keys, n_streams, n_kv_heads);
+}
+extern "C" int lcc_attn_decode_kv4(const void* q, void* out, const int32_t* slots, const int32_t* kv_len, void* const* kv_base, int n_slots, lcc_kv_layout lay, int layer,
+                                   int B, int n_q_heads, int nsplit, float* ws_o, float* ws_ml, void* stream) {
+  if (!q || !out || !slots || !kv_len || !kv_base) return fail(LCC_ERR_ARG, "lcc_attn_decode_kv4: null pointer");
+  if (not16(q) || not16(out) || not16(ws_o)) return fail(LCC_ERR_ALIGN, "lcc_attn_decode_kv4: pointers must be 16-byte aligned");
+  if (int rc = kv4_lay_ok(lay, "lcc_attn_decode_kv4")) return rc;
+  OP_RET(attn_decode_kv4(to_kv4(kv_base, n_slots, lay, layer), (const bf16_t*)q, slots, kv_len, B, n_q_heads, nsplit, ws_o, ws_ml, (bf16_t*)out, (hipStream_t)stream),
+         "lcc_attn_decode_kv4");
+}
+extern "C" int lcc_kv4_prefill_plan(const int32_t* n_new, const int32_t* past, int n_streams, int n_q_heads, int n_kv_heads, int cu_count, int32_t* tile_rows,
+                                    int32_t* nsplit) {
+  if (n_streams < 0 || (n_streams > 0 && (!n_new || !past)) || !tile_rows || !nsplit) return fail(LCC_ERR_ARG, "lcc_kv4_prefill_plan: bad argument");
+  const int rc = kv4_prefill_plan(n_new, past, n_streams, n_q_heads, n_kv_heads, cu_count, tile_rows, nsplit);
+  return rc ? fail(rc, "lcc_kv4_prefill_plan: invalid arguments (%d)", rc) : 0;
+}
+extern "C" int lcc_attn_prefill_kv4(const void* q, void* out, const int32_t* tile_stream, const int32_t* tile_q0, const int32_t* tile_nq, const int32_t* tile_pos0,
+                                    void* const* kv_base, int n_slots, lcc_kv_layout lay, int layer, int n_tiles, int n_q_heads, int tile_rows, int nsplit, int n_rows,
+                                    float* ws_o, float* ws_ml, void* stream) {
+  if (!q || !out || !tile_stream || !tile_q0 || !tile_nq || !tile_pos0 || !kv_base) return fail(LCC_ERR_ARG, "lcc_attn_prefill_kv4: null pointer");
+  if (not16(q) || not16(out) || not16(ws_o)) return fail(LCC_ERR_ALIGN, "lcc_attn_prefill_kv4: pointers must be 16-byte aligned");
+  if (int rc = kv4_lay_ok(lay, "lcc_attn_prefill_kv4")) return rc;
+  OP_RET(attn_prefill_kv4(to_kv4(kv_base, n_slots, lay, layer), (const bf16_t*)q, (bf16_t*)out, tile_stream, tile_q0, tile_nq, tile_pos0, n_tiles, n_q_heads, tile_rows,
+                          nsplit, n_rows, ws_o, ws_ml, (hipStream_t)stream), "lcc_attn_prefill_kv4");
+}

@@ -13,6 +13,7 @@
 // rpath $ORIGIN; loaded by livecc_amd/torch_ops.py (torch.ops.load_library).  The HF operator plugins (plugin.py) call through
 // torch.ops when the library is present.
 #include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
 
@@ -215,6 +216,126 @@ std::tuple<Tensor, Tensor> sample_greedy(const Tensor& logits, const Tensor& see
   return {out, scores};
 }
 
+// ---- KV cache in 4 bits: norm per head + rotation + append (also into the bf16 cache: the dtype of kv_buf says which), read-back, attention ----
+struct Cache { void* const* base; int n_slots; lcc_kv_layout lay; bool kv4; };
+Cache cache_of(const Tensor& like, const Tensor& kv_ptrs, const Tensor& kv_buf, int64_t n_layers, int64_t n_kv_heads, int64_t lmax, int64_t layer, bool bf16_too) {
+  chk(kv_ptrs, at::kLong, "kv_ptrs");
+  const bool kv4 = kv_buf.scalar_type() == at::kByte;
+  TORCH_CHECK(kv_buf.is_cuda() && kv_buf.is_contiguous() && kv_buf.dim() == 2 && (kv4 || (bf16_too && kv_buf.scalar_type() == at::kBFloat16)),
+              "kv_buf: contiguous uint8", bf16_too ? " or bf16" : "", " GPU tensor [n_slots, slot] expected");
+  TORCH_CHECK(kv_ptrs.device() == like.device() && kv_buf.device() == like.device(), "the cache must be on the device of the rows");
+  TORCH_CHECK(kv_ptrs.numel() == kv_buf.size(0), "kv_ptrs: one entry per slot expected");
+  TORCH_CHECK(n_layers >= 1 && n_kv_heads >= 1 && n_kv_heads <= 65535 && lmax >= 32 && lmax <= 0x7fffffe0 && (lmax % 32) == 0 && layer >= 0 && layer < n_layers,
+              "bad cache layout / layer");
+  const lcc_kv_layout lay = layout_of(n_layers, n_kv_heads, lmax);
+  const int64_t need = kv4 ? (int64_t)lcc_kv4_slot_bytes(lay) : n_layers * 2 * n_kv_heads * lmax * 128;
+  TORCH_CHECK(kv_buf.size(1) >= need, "kv_buf: a slot has ", kv_buf.size(1), " elements, the layout needs ", need);
+  return {(void* const*)kv_ptrs.data_ptr(), (int)kv_buf.size(0), lay, kv4};
+}
+void same_device(const Tensor& like, const Tensor& t, const char* name) { TORCH_CHECK(t.device() == like.device(), name, ": on ", t.device(), ", the rows are on ", like.device()); }
+const int32_t* index_ptr(const Tensor& like, const Tensor& t, int64_t n, bool at_least, const char* name) {
+  chk(t, at::kInt, name);
+  same_device(like, t, name);
+  TORCH_CHECK(at_least ? t.numel() >= n : t.numel() == n, name, ": ", n, at_least ? " or more" : "", " entries expected, got ", t.numel());
+  return (const int32_t*)t.data_ptr();
+}
+const int32_t* opt_index(const Tensor& like, const optional<Tensor>& t, int64_t n, bool at_least, const char* name) {
+  return t.has_value() && t->defined() ? index_ptr(like, *t, n, at_least, name) : nullptr;
+}
+const void* opt_vec(const Tensor& like, const optional<Tensor>& t, int64_t n, const char* name) {
+  const void* p = opt_ptr(t, at::kBFloat16, name);
+  if (p) { same_device(like, *t, name); TORCH_CHECK(t->numel() == n, name, ": ", n, " elements expected, got ", t->numel()); }
+  return p;
+}
+Tensor qk_norm_rope_kv_append(const optional<Tensor>& qkv, const optional<Tensor>& partial, const optional<Tensor>& bias, const optional<Tensor>& q_norm,
+                              const optional<Tensor>& k_norm, double eps, const Tensor& cos, const Tensor& sin, const Tensor& tok_stream,
+                              const optional<Tensor>& tok_pos, const optional<Tensor>& kv_len, const Tensor& kv_ptrs, Tensor& kv_buf, int64_t n_layers,
+                              int64_t n_kv_heads, int64_t lmax, int64_t layer, int64_t n_q_heads) {
+  chk(cos, at::kBFloat16, "cos"); chk(sin, at::kBFloat16, "sin");
+  TORCH_CHECK(cos.dim() == 2 && cos.size(1) == 64 && sin.sizes() == cos.sizes(), "qk_norm_rope_kv_append: cos / sin must be [S, 64]");
+  same_device(cos, sin, "sin");
+  const c10::DeviceGuard guard(cos.device());
+  const int64_t S = cos.size(0);
+  const Cache c = cache_of(cos, kv_ptrs, kv_buf, n_layers, n_kv_heads, lmax, layer, true);
+  const bool have_qkv = qkv.has_value() && qkv->defined(), have_part = partial.has_value() && partial->defined();
+  TORCH_CHECK(have_qkv != have_part, "qk_norm_rope_kv_append: exactly one of qkv (bf16 [S, (Hq+2Hkv)*128]) and partial (fp32 [NS, S, ...]) is needed");
+  TORCH_CHECK(n_q_heads >= 0 && n_q_heads <= 65535 && S <= 0x7fffffff, "qk_norm_rope_kv_append: bad n_q_heads / rows");
+  const int64_t width = (n_q_heads + 2 * n_kv_heads) * 128;
+  if (have_qkv) { TORCH_CHECK(qkv->dim() == 2 && qkv->size(0) == S && qkv->size(1) == width, "qk_norm_rope_kv_append: qkv must be [S, (Hq+2Hkv)*128]"); same_device(cos, *qkv, "qkv"); }
+  if (have_part) {
+    TORCH_CHECK(partial->dim() == 3 && partial->size(0) >= 1 && partial->size(0) <= 8 && partial->size(1) == S && partial->size(2) == width,
+                "qk_norm_rope_kv_append: partial must be [NS <= 8, S, (Hq+2Hkv)*128]");
+    same_device(cos, *partial, "partial");
+  }
+  const bool by_pos = tok_pos.has_value() && tok_pos->defined();
+  TORCH_CHECK(by_pos || (kv_len.has_value() && kv_len->defined()), "qk_norm_rope_kv_append: tok_pos or kv_len is needed");
+  const int32_t* strm = index_ptr(cos, tok_stream, S, false, "tok_stream");
+  const int32_t* pos = opt_index(cos, tok_pos, S, false, "tok_pos");
+  const int32_t* len = by_pos ? nullptr : opt_index(cos, kv_len, c.n_slots, true, "kv_len");
+  Tensor q = at::empty({S, n_q_heads * 128}, cos.options());
+  const auto call = c.kv4 ? lcc_qk_norm_rope_kv4_append : lcc_qk_norm_rope_kv_append_bf16;
+  if (S > 0)
+    ok(call(opt_ptr(qkv, at::kBFloat16, "qkv"), (const float*)opt_ptr(partial, at::kFloat, "partial"), have_part ? (int)partial->size(0) : 0,
+            opt_vec(cos, bias, width, "bias"), opt_vec(cos, q_norm, 128, "q_norm"), opt_vec(cos, k_norm, 128, "k_norm"), (float)eps, cos.data_ptr(), sin.data_ptr(), strm, pos,
+            len, c.base, c.n_slots, c.lay, (int)layer, n_q_heads > 0 ? q.data_ptr() : nullptr, (int)S, (int)n_q_heads, cur_stream(cos)),
+       c.kv4 ? "lcc_qk_norm_rope_kv4_append" : "lcc_qk_norm_rope_kv_append_bf16");
+  return q;
+}
+std::tuple<Tensor, Tensor> kv4_read(const Tensor& kv_ptrs, const Tensor& kv_buf, int64_t n_layers, int64_t n_kv_heads, int64_t lmax, int64_t layer, const Tensor& tok_stream,
+                                    const Tensor& tok_pos) {
+  const c10::DeviceGuard guard(tok_stream.device());
+  const int64_t S = tok_stream.numel();
+  TORCH_CHECK(S <= 0x7fffffff, "kv4_read: too many rows");
+  const int32_t *strm = index_ptr(tok_stream, tok_stream, S, false, "tok_stream"), *pos = index_ptr(tok_stream, tok_pos, S, false, "tok_pos");
+  const Cache c = cache_of(tok_stream, kv_ptrs, kv_buf, n_layers, n_kv_heads, lmax, layer, false);
+  Tensor k = at::empty({S, n_kv_heads, 128}, kv_buf.options().dtype(at::kBFloat16)), v = at::empty_like(k);
+  if (S > 0) ok(lcc_kv4_read(c.base, c.n_slots, c.lay, (int)layer, strm, pos, k.data_ptr(), v.data_ptr(), (int)S, cur_stream(kv_buf)), "lcc_kv4_read");
+  return {k, v};
+}
+Tensor attn_decode4(const Tensor& q, const Tensor& kv_ptrs, const Tensor& kv_buf, int64_t n_layers, int64_t n_kv_heads, int64_t lmax, int64_t layer, const Tensor& slots,
+                    const Tensor& kv_len, int64_t n_q_heads, int64_t nsplit) {
+  chk(q, at::kBFloat16, "q");
+  const c10::DeviceGuard guard(q.device());
+  const Cache c = cache_of(q, kv_ptrs, kv_buf, n_layers, n_kv_heads, lmax, layer, false);
+  TORCH_CHECK(n_q_heads >= 1 && n_q_heads % n_kv_heads == 0 && n_q_heads / n_kv_heads <= 16, "attn_decode4: up to 16 query heads per KV head");
+  TORCH_CHECK(q.dim() == 2 && q.size(1) == n_q_heads * 128 && q.size(0) <= 65535, "attn_decode4: q must be [B <= 65535, Hq*128]");
+  TORCH_CHECK(nsplit >= 1 && nsplit <= 64, "attn_decode4: nsplit must be 1..64");
+  const int64_t B = q.size(0);
+  const int32_t *sl = index_ptr(q, slots, B, false, "slots"), *len = index_ptr(q, kv_len, c.n_slots, true, "kv_len");
+  Tensor out = at::empty_like(q), ws;
+  float *ws_o = nullptr, *ws_ml = nullptr;
+  if (nsplit > 1) {
+    ws = at::empty({B * n_q_heads * nsplit * 130}, q.options().dtype(at::kFloat));
+    ws_o = (float*)ws.data_ptr(); ws_ml = ws_o + B * n_q_heads * nsplit * 128;
+  }
+  if (B > 0)
+    ok(lcc_attn_decode_kv4(q.data_ptr(), out.data_ptr(), sl, len, c.base, c.n_slots, c.lay, (int)layer, (int)B, (int)n_q_heads, (int)nsplit, ws_o, ws_ml, cur_stream(q)),
+       "lcc_attn_decode_kv4");
+  return out;
+}
+Tensor attn_prefill4(const Tensor& q, const Tensor& kv_ptrs, const Tensor& kv_buf, int64_t n_layers, int64_t n_kv_heads, int64_t lmax, int64_t layer, const Tensor& tiles,
+                     int64_t n_q_heads, int64_t tile_rows, int64_t nsplit) {
+  chk(q, at::kBFloat16, "q");
+  const c10::DeviceGuard guard(q.device());
+  const Cache c = cache_of(q, kv_ptrs, kv_buf, n_layers, n_kv_heads, lmax, layer, false);
+  TORCH_CHECK(n_q_heads >= 1 && n_q_heads % n_kv_heads == 0 && n_q_heads / n_kv_heads <= 16, "attn_prefill4: up to 16 query heads per KV head");
+  TORCH_CHECK(q.dim() == 2 && q.size(1) == n_q_heads * 128 && q.size(0) <= 0x7fffffff / n_q_heads, "attn_prefill4: q must be [S, Hq*128]");
+  TORCH_CHECK(tiles.dim() == 2 && tiles.size(0) == 4 && tiles.size(1) <= 65535, "attn_prefill4: tiles must be int32 [4, n <= 65535]: slot, first row, rows, first position");
+  TORCH_CHECK(tile_rows >= 1 && tile_rows <= 256 / (n_q_heads / n_kv_heads) && nsplit >= 1 && nsplit <= 32, "attn_prefill4: bad tile_rows / nsplit");
+  const int64_t S = q.size(0), nt = tiles.size(1);
+  const int32_t* t = index_ptr(q, tiles, 4 * nt, false, "tiles");
+  Tensor out = at::empty_like(q), ws;
+  float *ws_o = nullptr, *ws_ml = nullptr;
+  if (nsplit > 1) {
+    ws = at::empty({S * n_q_heads * nsplit * 130}, q.options().dtype(at::kFloat));
+    ws_o = (float*)ws.data_ptr(); ws_ml = ws_o + S * n_q_heads * nsplit * 128;
+  }
+  if (S > 0)
+    ok(lcc_attn_prefill_kv4(q.data_ptr(), out.data_ptr(), t, t + nt, t + 2 * nt, t + 3 * nt, c.base, c.n_slots, c.lay, (int)layer, (int)nt, (int)n_q_heads, (int)tile_rows,
+                            (int)nsplit, (int)S, ws_o, ws_ml, cur_stream(q)), "lcc_attn_prefill_kv4");
+  return out;
+}
+
 }  // namespace
 
 TORCH_LIBRARY(livecc_amd, m) {
@@ -233,6 +354,13 @@ TORCH_LIBRARY(livecc_amd, m) {
         "Tensor wy, int ky) -> Tensor");
   m.def("sample_greedy(Tensor logits, Tensor(a!) seen, Tensor slots, float repetition_penalty, int thr_token, bool use_thr, float thr_value, "
         "int eos_token, int eos_token2, bool suppress_eos, bool want_scores) -> (Tensor, Tensor)");
+  m.def("qk_norm_rope_kv_append(Tensor? qkv, Tensor? partial, Tensor? bias, Tensor? q_norm, Tensor? k_norm, float eps, Tensor cos, Tensor sin, Tensor tok_stream, "
+        "Tensor? tok_pos, Tensor? kv_len, Tensor kv_ptrs, Tensor(a!) kv_buf, int n_layers, int n_kv_heads, int lmax, int layer, int n_q_heads) -> Tensor");
+  m.def("kv4_read(Tensor kv_ptrs, Tensor kv_buf, int n_layers, int n_kv_heads, int lmax, int layer, Tensor tok_stream, Tensor tok_pos) -> (Tensor, Tensor)");
+  m.def("attn_decode4(Tensor q, Tensor kv_ptrs, Tensor kv_buf, int n_layers, int n_kv_heads, int lmax, int layer, Tensor slots, Tensor kv_len, int n_q_heads, "
+        "int nsplit) -> Tensor");
+  m.def("attn_prefill4(Tensor q, Tensor kv_ptrs, Tensor kv_buf, int n_layers, int n_kv_heads, int lmax, int layer, Tensor tiles, int n_q_heads, int tile_rows, "
+        "int nsplit) -> Tensor");
 }
 
 // device key "CUDA" is the HIP device key of PyTorch-ROCm (c10::DispatchKey::CUDA == HIP builds' GPU key)
@@ -247,4 +375,8 @@ TORCH_LIBRARY_IMPL(livecc_amd, CUDA, m) {
   m.impl("patchify_norm", &patchify_norm);
   m.impl("resize_bicubic_aa", &resize_bicubic_aa);
   m.impl("sample_greedy", &sample_greedy);
+  m.impl("qk_norm_rope_kv_append", &qk_norm_rope_kv_append);
+  m.impl("kv4_read", &kv4_read);
+  m.impl("attn_decode4", &attn_decode4);
+  m.impl("attn_prefill4", &attn_prefill4);
 }

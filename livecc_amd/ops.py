@@ -421,6 +421,208 @@ def attn_decode(q: torch.Tensor, kv: KvArena, layer: int, slots: torch.Tensor, k
     return out
 
 
+# ---- KV cache in 4 bits (csrc/kv4.hip) ----
+_KV4_VALUES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+class Kv4Arena:
+    """Stand-alone 4-bit KV arena(s): groups of 32 channels of one token and KV head share a power of two, 4.25 bits a value (include/livecc_amd.h
+    has the format and the layout).  Slots, layers, heads and capacity as `KvArena`; `k_view` / `v_view` are bf16 copies of the values held."""
+
+    def __init__(self, n_slots, n_layers, n_kv_heads, lmax, device):
+        self.lay = _lib.KvLayout(n_layers, n_kv_heads, lmax, 128)
+        self.per_slot = _lib.load().lcc_kv4_slot_bytes(self.lay)
+        if self.per_slot == 0:
+            raise ValueError(f"Kv4Arena: {_lib.load().lcc_last_error().decode(errors='replace')}")
+        self.buf = torch.zeros(n_slots, self.per_slot, dtype=torch.uint8, device=device)
+        ptrs = self.buf.data_ptr() + np.arange(n_slots, dtype=np.int64) * self.per_slot
+        self.ptrs = torch.as_tensor(ptrs, device=device)
+        self.n_kv_heads, self.lmax, self.n_layers = n_kv_heads, lmax, n_layers
+
+    def _layer(self, slot, layer):
+        c, s = self.n_kv_heads * self.lmax * 64, self.n_kv_heads * self.lmax * 4
+        n = 2 * (c + s)
+        return self.buf[slot, layer * n:(layer + 1) * n].split((c, c, s, s))
+
+    @staticmethod
+    def _values(halves, e):                        # [..., 128] codes, [..., 4] scales
+        table = torch.tensor(_KV4_VALUES + tuple(-v for v in _KV4_VALUES), device=halves.device)
+        scale = torch.where(e == 255, float("nan"), torch.ldexp(torch.ones((), device=e.device), e.int() - 127))
+        return (table[halves.int()].unflatten(-1, (4, 32)) * scale.unsqueeze(-1)).flatten(-2).to(torch.bfloat16)
+
+    def k_view(self, slot, layer):  # [Hkv, Lmax, 128]
+        kc, _, ks, _ = self._layer(slot, layer)
+        kc = kc.view(self.n_kv_heads, self.lmax, 64)
+        return self._values(torch.stack((kc & 15, kc >> 4), -1).flatten(-2), ks.view(self.n_kv_heads, self.lmax, 4))
+
+    def v_view(self, slot, layer):  # [Hkv, Lmax, 128]
+        _, vc, _, vs = self._layer(slot, layer)
+        vc = vc.view(self.n_kv_heads, self.lmax // 32, 4, 16, 4, 8)                       # head, block, g, i, t, e
+        halves = torch.stack((vc & 15, vc >> 4), -1).permute(0, 1, 2, 5, 4, 6, 3)          # head, block, g, e, t, half, i
+        scales = vs.view(self.n_kv_heads, self.lmax // 32, 4, 4, 8).permute(0, 1, 2, 4, 3)
+        return self._values(halves.reshape(self.n_kv_heads, self.lmax, 128), scales.reshape(self.n_kv_heads, self.lmax, 4))
+
+
+def qk_norm_rope_kv_append(qkv: Optional[torch.Tensor], cos, sin, tok_stream, tok_pos, kv, layer: int, n_q_heads: int, q_norm: Optional[torch.Tensor] = None,
+                           k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6, partial: Optional[torch.Tensor] = None,
+                           bias: Optional[torch.Tensor] = None, kv_len: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """`rope_kv_append` with RMS norms of the query and key heads (weights [128], None: no norm) in front of the rotation, into a `KvArena` or a `Kv4Arena`;
+    returns the queries [S, Hq*128].  A row whose `tok_stream` is out of range (-1: padding) or whose position is behind the arena appends nothing.  (slot,
+    position) pairs of a call must be distinct."""
+    for a, dt, nm in ((qkv, torch.bfloat16, "qkv"), (partial, torch.float32, "partial"), (cos, torch.bfloat16, "cos"), (tok_stream, torch.int32, "tok_stream")):
+        _chk(a, dt, nm)
+    if cos.shape[0] == 0 or (q_norm is None and k_norm is None) or eps > 0:
+        t = _T.op("qk_norm_rope_kv_append")
+        if t is not None:
+            return t(qkv, partial, bias, q_norm, k_norm, float(eps), cos, sin, tok_stream, tok_pos, kv_len, kv.ptrs, kv.buf, kv.n_layers, kv.n_kv_heads, kv.lmax,
+                     int(layer), int(n_q_heads))
+    else:
+        raise ValueError("qk_norm_rope_kv_append: eps must be positive")
+    S, width = cos.shape[0], (n_q_heads + 2 * kv.n_kv_heads) * 128
+    n_slots = kv.buf.shape[0]
+    _same_device(cos, sin=sin, tok_stream=tok_stream, tok_pos=tok_pos, kv_len=kv_len, qkv=qkv, partial=partial, bias=bias, q_norm=q_norm, k_norm=k_norm, kv=kv.buf)
+    _shape(cos, (S, 64), "cos"), _shape(sin, (S, 64), "sin"), _shape(tok_stream, (S,), "tok_stream")
+    if tok_pos is not None:
+        _shape(tok_pos, (S,), "tok_pos")
+    elif kv_len is None or kv_len.numel() < n_slots:
+        raise ValueError("qk_norm_rope_kv_append: tok_pos, or kv_len of every slot, is needed")
+    for a, shape, nm in ((qkv, (S, width), "qkv"), (partial, (0 if partial is None else partial.shape[0], S, width), "partial"), (bias, (width,), "bias"),
+                         (q_norm, (128,), "q_norm"), (k_norm, (128,), "k_norm")):
+        if a is not None:
+            _shape(a, shape, nm)
+    q = torch.empty(S, n_q_heads * 128, dtype=torch.bfloat16, device=cos.device)
+    if S == 0:
+        return q
+    lib, name = _lib.load(), "lcc_qk_norm_rope_kv4_append" if isinstance(kv, Kv4Arena) else "lcc_qk_norm_rope_kv_append_bf16"
+    with torch.cuda.device(cos.device):
+        _lib.check(getattr(lib, name)(
+            _chk(qkv, torch.bfloat16, "qkv"), _chk(partial, torch.float32, "partial"), partial.shape[0] if partial is not None else 0, _chk(bias, torch.bfloat16, "bias"),
+            _chk(q_norm, torch.bfloat16, "q_norm"), _chk(k_norm, torch.bfloat16, "k_norm"), float(eps), _chk(cos, torch.bfloat16, "cos"), _chk(sin, torch.bfloat16, "sin"),
+            _chk(tok_stream, torch.int32, "tok_stream"), _chk(tok_pos, torch.int32, "tok_pos"), _chk(kv_len, torch.int32, "kv_len"), kv.ptrs.data_ptr(), n_slots, kv.lay,
+            int(layer), q.data_ptr() if n_q_heads > 0 else None, S, int(n_q_heads), _st(cos)), name)
+    return q
+
+
+def _same_device(like: torch.Tensor, **others) -> None:
+    for name, t in others.items():
+        if t is not None and t.device != like.device:
+            raise ValueError(f"{name}: on {t.device}, the rows are on {like.device}")
+
+
+def _shape(t: torch.Tensor, shape, name: str) -> None:
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name}: shape {tuple(shape)} expected, got {tuple(t.shape)}")
+
+
+def _kv4(kv) -> None:
+    if not isinstance(kv, Kv4Arena):
+        raise TypeError(f"kv: a Kv4Arena expected, got {type(kv).__name__}")
+
+
+def kv4_read(kv: Kv4Arena, layer: int, tok_stream: torch.Tensor, tok_pos: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Keys and values [S, Hkv, 128] (bf16) of S (slot, position) pairs out of the 4-bit cache; zeros where a pair is out of range."""
+    _kv4(kv)
+    _chk(tok_stream, torch.int32, "tok_stream"), _chk(tok_pos, torch.int32, "tok_pos")
+    t = _T.op("kv4_read")
+    if t is not None:
+        return t(kv.ptrs, kv.buf, kv.n_layers, kv.n_kv_heads, kv.lmax, int(layer), tok_stream, tok_pos)
+    S = tok_stream.numel()
+    _same_device(tok_stream, tok_pos=tok_pos, kv=kv.buf), _shape(tok_stream, (S,), "tok_stream"), _shape(tok_pos, (S,), "tok_pos")
+    k = torch.empty(S, kv.n_kv_heads, 128, dtype=torch.bfloat16, device=kv.buf.device)
+    v = torch.empty_like(k)
+    if S > 0:
+        with torch.cuda.device(k.device):
+            _lib.check(_lib.load().lcc_kv4_read(kv.ptrs.data_ptr(), kv.buf.shape[0], kv.lay, int(layer), tok_stream.data_ptr(), tok_pos.data_ptr(), k.data_ptr(), v.data_ptr(), S,
+                                                _st(k)), "lcc_kv4_read")
+    return k, v
+
+
+def kv4_decode_splits(n_keys: Sequence[int], n_kv_heads: int) -> int:
+    """Key splits that suit one `attn_decode4` launch for streams of n_keys keys each, the new ones included (lcc_kv4_decode_splits: host logic, no GPU)."""
+    n = np.ascontiguousarray(np.asarray(list(n_keys), dtype=np.int32))
+    rc = _lib.load().lcc_kv4_decode_splits(n.ctypes.data, int(n.size), int(n_kv_heads))
+    if rc < 0:
+        _lib.check(rc, "lcc_kv4_decode_splits")
+    return rc
+
+
+def attn_decode4(q: torch.Tensor, kv: Kv4Arena, layer: int, slots: torch.Tensor, kv_len: torch.Tensor, n_q_heads: int, nsplit: int = 0) -> torch.Tensor:
+    """`attn_decode` over the 4-bit cache: row b sees keys 0 .. kv_len[slots[b]] of its slot (none at -1, or for a slot out of range: zeros).  nsplit 0: the split
+    count that suits streams as long as the arena; callers that know the lengths take it from `kv4_decode_splits`."""
+    _kv4(kv)
+    _chk(q, torch.bfloat16, "q"), _chk(slots, torch.int32, "slots"), _chk(kv_len, torch.int32, "kv_len")
+    if nsplit == 0:
+        nsplit = kv4_decode_splits([kv.lmax] * max(1, q.shape[0]), kv.n_kv_heads)
+    t = _T.op("attn_decode4")
+    if t is not None:
+        return t(q, kv.ptrs, kv.buf, kv.n_layers, kv.n_kv_heads, kv.lmax, int(layer), slots, kv_len, int(n_q_heads), int(nsplit))
+    B, n_slots = q.shape[0], kv.buf.shape[0]
+    _same_device(q, slots=slots, kv_len=kv_len, kv=kv.buf), _shape(q, (B, n_q_heads * 128), "q"), _shape(slots, (B,), "slots")
+    if kv_len.numel() < n_slots:
+        raise ValueError("kv_len: one entry per slot expected")
+    out = torch.empty_like(q)
+    if B > 0:
+        ws = torch.empty(B * n_q_heads * nsplit * 130, dtype=torch.float32, device=q.device) if nsplit > 1 else None
+        with torch.cuda.device(q.device):
+            _lib.check(_lib.load().lcc_attn_decode_kv4(q.data_ptr(), out.data_ptr(), slots.data_ptr(), kv_len.data_ptr(), kv.ptrs.data_ptr(), n_slots, kv.lay, int(layer), B,
+                                                       int(n_q_heads), int(nsplit), None if ws is None else ws.data_ptr(),
+                                                       None if ws is None else ws.data_ptr() + B * n_q_heads * nsplit * 512, _st(q)), "lcc_attn_decode_kv4")
+    return out
+
+
+class Kv4PrefillPlan:
+    """Launch plan of `attn_prefill4`: made once for a call's segments, used for every layer."""
+
+    def __init__(self, segments: Sequence[Tuple[int, int, int]], n_q_heads: int, n_kv_heads: int, device, nsplit: int = 0):
+        seg = np.asarray(list(segments), dtype=np.int32).reshape(-1, 3)
+        new, past = np.ascontiguousarray(seg[:, 1]), np.ascontiguousarray(seg[:, 2])
+        device = torch.device(device)
+        cus = torch.cuda.get_device_properties(device).multi_processor_count if device.type == "cuda" else 256
+        plan = np.zeros(2, dtype=np.int32)
+        _lib.check(_lib.load().lcc_kv4_prefill_plan(new.ctypes.data, past.ctypes.data, len(seg), int(n_q_heads), int(n_kv_heads), cus, plan[0:].ctypes.data,
+                                                    plan[1:].ctypes.data), "lcc_kv4_prefill_plan")
+        self.tile_rows, self.nsplit = int(plan[0]), int(nsplit) if nsplit > 0 else int(plan[1])
+        self.n_q_heads, self.n_kv_heads, self.rows = int(n_q_heads), int(n_kv_heads), int(new.sum())
+        self.max_keys = int((new.astype(np.int64) + past)[new > 0].max(initial=0))
+        tiles, row = [], 0
+        for slot, n, p in seg.tolist():
+            tiles += [(slot, row + o, min(self.tile_rows, n - o), p + o) for o in range(0, n, self.tile_rows)]
+            row += n
+        self.tiles = torch.as_tensor(np.ascontiguousarray(np.asarray(tiles, dtype=np.int32).reshape(-1, 4).T), device=device)
+
+
+def kv4_prefill_plan(segments: Sequence[Tuple[int, int, int]], n_q_heads: int, n_kv_heads: int, device, nsplit: int = 0) -> Kv4PrefillPlan:
+    """segments: (slot, n_new, past_len) per stream, rows packed in that order.  nsplit 0: the split count that suits them (lcc_kv4_prefill_plan)."""
+    return Kv4PrefillPlan(segments, n_q_heads, n_kv_heads, device, nsplit)
+
+
+def attn_prefill4(q: torch.Tensor, kv: Kv4Arena, layer: int, plan, n_q_heads: int) -> torch.Tensor:
+    """`attn_prefill` over the 4-bit cache; plan: a `kv4_prefill_plan`, or the segments themselves.  A row at position p sees keys 0 .. p of its slot (a slot out of
+    range: zeros)."""
+    _kv4(kv)
+    if not isinstance(plan, Kv4PrefillPlan):
+        plan = Kv4PrefillPlan(plan, n_q_heads, kv.n_kv_heads, q.device)
+    _chk(q, torch.bfloat16, "q"), _chk(plan.tiles, torch.int32, "plan")
+    if plan.rows != q.shape[0] or plan.n_q_heads != n_q_heads or plan.n_kv_heads != kv.n_kv_heads:
+        raise ValueError(f"attn_prefill4: the plan is of {plan.rows} rows, {plan.n_q_heads} / {plan.n_kv_heads} heads")
+    if plan.max_keys > kv.lmax:
+        raise ValueError(f"attn_prefill4: {plan.max_keys} keys, the arena holds {kv.lmax}")
+    t = _T.op("attn_prefill4")
+    if t is not None:
+        return t(q, kv.ptrs, kv.buf, kv.n_layers, kv.n_kv_heads, kv.lmax, int(layer), plan.tiles, int(n_q_heads), plan.tile_rows, plan.nsplit)
+    S, nt = q.shape[0], plan.tiles.shape[1]
+    _same_device(q, plan=plan.tiles, kv=kv.buf), _shape(q, (S, n_q_heads * 128), "q")
+    out = torch.empty_like(q)
+    if S > 0:
+        ws = torch.empty(S * n_q_heads * plan.nsplit * 130, dtype=torch.float32, device=q.device) if plan.nsplit > 1 else None
+        at = plan.tiles.data_ptr()
+        with torch.cuda.device(q.device):
+            _lib.check(_lib.load().lcc_attn_prefill_kv4(q.data_ptr(), out.data_ptr(), at, at + 4 * nt, at + 8 * nt, at + 12 * nt, kv.ptrs.data_ptr(), kv.buf.shape[0], kv.lay,
+                                                        int(layer), nt, int(n_q_heads), plan.tile_rows, plan.nsplit, S, None if ws is None else ws.data_ptr(),
+                                                        None if ws is None else ws.data_ptr() + S * n_q_heads * plan.nsplit * 512, _st(q)), "lcc_attn_prefill_kv4")
+    return out
+
+
 def embed_gather(ids: torch.Tensor, table: torch.Tensor, vit_index: Optional[torch.Tensor] = None,
                  vit_rows: Optional[torch.Tensor] = None, indirect: Optional[torch.Tensor] = None, n_rows: Optional[int] = None):
     """`embed_tokens(input_ids)` + `masked_scatter` of the video rows (Q2VL:1159-1176) in one pass: row s of the result is

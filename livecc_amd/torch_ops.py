@@ -3,7 +3,8 @@
 The C-ABI (include/livecc_amd.h) stays the source of truth -- the registered ops forward to the same `lcc_*` symbols on
 `c10::hip::getCurrentHIPStream()` with `TORCH_CHECK` validation -- but unlike ctypes-on-`data_ptr()` they are visible to the
 dispatcher: profiler ranges, schema-checked arguments, mutation annotations, TorchScript / export.  `livecc_amd.ops` routes
-`rmsnorm / layernorm / swiglu / linear / rope_kv_append / attn_prefill / attn_decode / patchify_norm / sample_greedy` and
+`rmsnorm / layernorm / swiglu / linear / rope_kv_append / attn_prefill / attn_decode / patchify_norm / sample_greedy /
+qk_norm_rope_kv_append / kv4_read / attn_decode4 / attn_prefill4` and
 `livecc_amd.resize.resize_bicubic_aa` through them when the library is present (LCC_TORCH_OPS=0: ctypes only), so the HF operator
 plugins (`plugin.py`) run through `torch.ops`.  No CPU kernels are registered: a CPU tensor raises NotImplementedError.
 """
@@ -15,7 +16,7 @@ from collections import Counter
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "_C", "liblivecc_torch_ops.so")
 OP_NAMES = ("rmsnorm", "layernorm", "swiglu", "linear", "rope_kv_append", "attn_prefill", "attn_decode", "patchify_norm",
-            "resize_bicubic_aa", "sample_greedy")
+            "resize_bicubic_aa", "sample_greedy", "qk_norm_rope_kv_append", "kv4_read", "attn_decode4", "attn_prefill4")
 CALLS: Counter = Counter()          # calls routed through torch.ops per op name (tests assert that the dispatcher path really ran)
 _ns = None
 _tried = False

@@ -1,0 +1,528 @@
+"""GPU tests of the 4-bit KV cache (livecc_amd/csrc/kv4.hip): norm + rotation + append into both caches, read-back, attention of tokens and of chunks,
+each against plain 64-bit forms (tests/kv4_util.py), and a run of them as a decoder layer would use them."""
+import math
+
+import pytest
+import torch
+
+from tests import kv4_util as U
+
+pytestmark = pytest.mark.gpu
+
+
+def rand(shape, dev, seed, scale=1.0):
+    g = torch.Generator(device="cpu").manual_seed(seed)
+    return (torch.randn(shape, generator=g) * scale).to(torch.bfloat16).to(dev)
+
+
+def i32(v, dev):
+    return torch.tensor(v, dtype=torch.int32, device=dev)
+
+
+def tables(pos, dev):
+    at = torch.tensor(pos, dtype=torch.float64).clamp(min=0)[:, None] * 1e4 ** (-torch.arange(64, dtype=torch.float64) / 64)
+    return at.cos().to(torch.bfloat16).to(dev), at.sin().to(torch.bfloat16).to(dev)
+
+
+def filled(dev, k, v, layers=1, layer=0):
+    """a Kv4Arena whose slots hold k, v [n, Hkv, L, 128] (through the append kernel: it has tests of its own), and the values held"""
+    from livecc_amd import ops
+    n, hkv, L, _ = k.shape
+    kv = ops.Kv4Arena(n, layers, hkv, (L + 31) // 32 * 32, dev)
+    rows = torch.cat((k.permute(0, 2, 1, 3).reshape(n * L, hkv * 128), v.permute(0, 2, 1, 3).reshape(n * L, hkv * 128)), 1).contiguous()
+    one = torch.ones(n * L, 64, dtype=torch.bfloat16, device=dev)
+    stream = torch.arange(n, device=dev, dtype=torch.int32).repeat_interleave(L)
+    pos = torch.arange(L, device=dev, dtype=torch.int32).repeat(n)
+    ops.qk_norm_rope_kv_append(rows, one, torch.zeros_like(one), stream, pos, kv, layer, 0)
+    return kv
+
+
+def values(kv, slot, layer=0):
+    return kv.k_view(slot, layer).double().cpu(), kv.v_view(slot, layer).double().cpu()
+
+
+# ---- append
+@pytest.mark.parametrize("heads,kv_heads", [(2, 1), (28, 4), (8, 8), (32, 2)])
+@pytest.mark.parametrize("rows,past", [(1, 0), (1, 31), (7, 30), (33, 1), (70, 29)])
+@pytest.mark.parametrize("norm", ["both", "q", "k", "none"])
+@pytest.mark.parametrize("bits", [16, 4])
+def test_norm_rope_append(dev, heads, kv_heads, rows, past, norm, bits):
+    """Every value and every code equals the definition's: the one step that is not exact, the root of a 64-bit mean rounded once to fp32, differs only where the
+    mean's last bits decide (2^-28 of the cases).  Untouched positions and other layers stay as they were."""
+    from livecc_amd import ops
+    n, lmax, layers, layer = 3, 128, 2, 1
+    S = n * rows
+    qkv = rand((S, (heads + 2 * kv_heads) * 128), dev, 1, 2.0)
+    qkv[0, :128] = 0
+    qn, kn = rand((128,), dev, 2) if norm in ("both", "q") else None, rand((128,), dev, 3) if norm in ("both", "k") else None
+    pos = [past + s + r for s in range(n) for r in range(rows)]
+    stream = [s for s in (2, 0, 1) for _ in range(rows)]
+    pos = [min(p, lmax - 1 - (S - i)) if p >= lmax else p for i, p in enumerate(pos)]
+    cos, sin = tables(pos, dev)
+    kv = (ops.Kv4Arena if bits == 4 else ops.KvArena)(n, layers, kv_heads, lmax, dev)
+    kv.buf.view(torch.uint8).fill_(0x3B)
+    before = kv.buf.clone()
+    q = ops.qk_norm_rope_kv_append(qkv, cos, sin, i32(stream, dev), i32(pos, dev), kv, layer, heads, q_norm=qn, k_norm=kn)
+    x = qkv.cpu().view(S, heads + 2 * kv_heads, 128)
+    c, s = cos.cpu(), sin.cpu()
+    want_q = U.norm_rope(x[:, :heads], None if qn is None else qn.cpu(), c, s)
+    want_k = U.norm_rope(x[:, heads:heads + kv_heads], None if kn is None else kn.cpu(), c, s)
+    want_v = x[:, heads + kv_heads:].double()
+    assert torch.equal(q.double().cpu().view_as(want_q), want_q)
+    if bits == 4:
+        want_k, want_v = U.quantise(want_k)[2], U.quantise(want_v)[2]
+    for i, (sl, p) in enumerate(zip(stream, pos)):
+        assert torch.equal(kv.k_view(sl, layer)[:, p].double().cpu(), want_k[i]), (sl, p)
+        assert torch.equal(kv.v_view(sl, layer)[:, p].double().cpu(), want_v[i]), (sl, p)
+    # nothing else changed: put back what was written and compare all bytes
+    same = kv.buf.clone()
+    per = kv.buf.shape[1] // layers
+    assert torch.equal(same[:, :per], before[:, :per])
+    changed = (kv.buf != before).sum().item()
+    most = S * kv_heads * (136 if bits == 4 else 256)
+    assert changed <= most
+
+
+def test_append_without_norms_equals_the_existing_append(dev):
+    from livecc_amd import ops
+    heads, kv_heads, rows = 28, 4, 45
+    qkv = rand((rows, 36 * 128), dev, 5)
+    pos = list(range(9, 9 + rows))
+    cos, sin = tables(pos, dev)
+    a, b = ops.KvArena(1, 1, kv_heads, 64, dev), ops.KvArena(1, 1, kv_heads, 64, dev)
+    st = i32([0] * rows, dev)
+    qa = ops.rope_kv_append(qkv, cos, sin, st, i32(pos, dev), a, 0, heads)
+    qb = ops.qk_norm_rope_kv_append(qkv, cos, sin, st, i32(pos, dev), b, 0, heads)
+    assert torch.equal(qa, qb) and torch.equal(a.buf, b.buf)
+
+
+@pytest.mark.parametrize("nsplit", [1, 3, 8])
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("with_bias", [True, False])
+def test_append_from_slabs(dev, nsplit, bits, with_bias):
+    """fp32 slabs, summed in order, plus the bias, rounded: as the bf16 rows with that value."""
+    from livecc_amd import ops
+    heads, kv_heads, S = 7, 1, 5
+    g = torch.Generator().manual_seed(nsplit)
+    part = torch.randn(nsplit, S, 9 * 128, generator=g).to(dev)
+    bias = rand((9 * 128,), dev, 4) if with_bias else None
+    acc = torch.zeros_like(part[0])
+    for p in part:
+        acc = acc + p
+    qkv = (acc + bias.float() if with_bias else acc).to(torch.bfloat16)
+    cos, sin = tables(range(S), dev)
+    kn = rand((128,), dev, 8)
+    out = []
+    for src in ("rows", "slabs"):
+        kv = (ops.Kv4Arena if bits == 4 else ops.KvArena)(2, 1, kv_heads, 32, dev)
+        q = ops.qk_norm_rope_kv_append(qkv if src == "rows" else None, cos, sin, i32([1, 0, 1, 1, 0], dev), i32([3, 4, 5, 6, 31], dev), kv, 0, heads,
+                                       q_norm=kn, k_norm=kn, partial=None if src == "rows" else part, bias=None if src == "rows" else bias)
+        out.append((q, kv.buf))
+    assert torch.equal(out[0][0], out[1][0]) and torch.equal(out[0][1], out[1][1])
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_append_at_kv_len_and_rows_of_no_stream(dev, bits):
+    """tok_pos None: positions are the slots' lengths.  Rows of stream -1, of a stream that does not exist, and streams whose position is out of range: queries come, the
+    cache stays."""
+    from livecc_amd import ops
+    heads, kv_heads, S, n = 4, 2, 7, 4
+    qkv = rand((S, 8 * 128), dev, 6)
+    cos, sin = tables([1] * S, dev)
+    stream, lens = [2, -1, 0, 9, 1, 3, -5], [31, 64, 17, -1]
+    kv = (ops.Kv4Arena if bits == 4 else ops.KvArena)(n, 1, kv_heads, 64, dev)
+    q = ops.qk_norm_rope_kv_append(qkv, cos, sin, i32(stream, dev), None, kv, 0, heads, kv_len=i32(lens, dev))
+    x = qkv.cpu().view(S, 8, 128)
+    want = U.norm_rope(x[:, :heads], None, cos.cpu(), sin.cpu())
+    assert torch.equal(q.double().cpu().view_as(want), want)
+    k = U.norm_rope(x[:, heads:heads + kv_heads], None, cos.cpu(), sin.cpu())
+    k = U.quantise(k)[2] if bits == 4 else k
+    for slot in range(n):
+        held = kv.k_view(slot, 0).double().cpu()
+        for row, p in {2: ((0, 17),), 0: ((2, 31),)}.get(slot, ()):
+            assert torch.equal(held[:, p], k[row])
+            held[:, p] = 0
+        assert not held.any() and (slot in (0, 2) or not kv.buf[slot].any())
+
+
+def test_codes_of_every_bf16(dev):
+    """Groups whose largest magnitude is each of the finite bf16 magnitudes in turn, beside values spread over its binades, zeros, and both signs; infinities and NaN."""
+    from livecc_amd import ops
+    bits = torch.arange(0, 0x7F80, 61, dtype=torch.int32)
+    a = bits.to(torch.int16).view(torch.bfloat16).double()
+    rows = len(a)
+    g = torch.Generator().manual_seed(0)
+    frac = torch.rand(rows, 256, generator=g, dtype=torch.float64) * 2 - 1
+    frac[:, ::7] = torch.round(frac[:, ::7] * 16) / 16                       # many ties
+    frac[:, 0::32] = 1.0
+    frac[:, 5::32] = 0.0
+    x = (a[:, None] * frac).to(torch.bfloat16)
+    x = torch.where(x.double().abs() > a[:, None], x.sign() * a[:, None].to(torch.bfloat16), x)
+    x[3, 40], x[5, 200], x[9, 130] = math.inf, -math.inf, math.nan
+    kv = ops.Kv4Arena(1, 1, 1, (rows + 31) // 32 * 32, dev)
+    one = torch.ones(rows, 64, dtype=torch.bfloat16, device=dev)
+    # keys through the identity rotation x * 1 - y * 0: an infinity beside it would become a NaN there, which the group is in any case
+    ops.qk_norm_rope_kv_append(x.to(dev), one, torch.zeros_like(one), torch.zeros(rows, dtype=torch.int32, device=dev), torch.arange(rows, dtype=torch.int32, device=dev), kv, 0, 0)
+    rot = x[:, :128].double()
+    rot = torch.cat((rot[:, :64] - rot[:, 64:] * 0, rot[:, 64:] + rot[:, :64] * 0), 1)
+    want_k, want_v = U.quantise(rot)[2], U.quantise(x[:, 128:])[2]
+    for want, got in ((want_k, kv.k_view(0, 0)), (want_v, kv.v_view(0, 0))):
+        got = got[0, :rows].double().cpu()
+        assert torch.equal(torch.isnan(got), torch.isnan(want))
+        assert torch.equal(got.nan_to_num(0.0), want.nan_to_num(0.0))
+        # and the format's own promise: off by at most half of its largest step, that is one scale, of which 3.5 are below the largest magnitude (where no clamp applies)
+        src = (rot if want is want_k else x[:, 128:].double()).unflatten(-1, (4, 32))
+        err, top = (want.unflatten(-1, (4, 32)) - src).abs(), src.abs().amax(-1, keepdim=True)
+        sane = (torch.isfinite(top) & (top > 2.0 ** -120) & (top < 2.0 ** 127)).expand_as(err)
+        assert bool((err <= top / 3.5)[sane].all())
+
+
+@pytest.mark.parametrize("kv_heads,lmax", [(1, 32), (4, 96)])
+def test_read_back(dev, kv_heads, lmax):
+    from livecc_amd import ops
+    k, v = rand((3, kv_heads, lmax, 128), dev, 1), rand((3, kv_heads, lmax, 128), dev, 2)
+    v[1, 0, 3, 70] = math.nan
+    kv = filled(dev, k, v, layers=2, layer=1)
+    stream = [0, 2, 1, -1, 3, 1, 1, 0, 2]
+    pos = [0, lmax - 1, 3, 3, 3, -1, lmax, 17, 31]
+    gk, gv = ops.kv4_read(kv, 1, i32(stream, dev), i32(pos, dev))
+    for i, (s, p) in enumerate(zip(stream, pos)):
+        if 0 <= s < 3 and 0 <= p < lmax:
+            assert torch.equal(gk[i], kv.k_view(s, 1)[:, p])
+            assert torch.equal(gv[i].nan_to_num(9.0), kv.v_view(s, 1)[:, p].nan_to_num(9.0))
+        else:
+            assert not gk[i].any() and not gv[i].any()
+
+
+# ---- attention of single tokens
+@pytest.mark.parametrize("heads,kv_heads", [(2, 1), (7, 1), (28, 4), (3, 3), (32, 2)])
+@pytest.mark.parametrize("nsplit", [1, 2, 5])
+def test_decode(dev, heads, kv_heads, nsplit):
+    from livecc_amd import ops
+    L, n = 224, 4
+    k, v = rand((n, kv_heads, L, 128), dev, 1), rand((n, kv_heads, L, 128), dev, 2)
+    kv = filled(dev, k, v)
+    lens = [0, 31, 32, 223]
+    slots = [3, 0, 2, 1, 2]
+    q = rand((len(slots), heads * 128), dev, 3)
+    got = ops.attn_decode4(q, kv, 0, i32(slots, dev), i32(lens, dev), heads, nsplit)
+    for i, s in enumerate(slots):
+        kk, vv = values(kv, s)
+        want, tol = U.attention(q[i:i + 1].cpu().view(1, heads, 128), kk, vv, [lens[s]])
+        U.assert_within(got[i], want[0].flatten(), tol[0].flatten(), f"row {i}, length {lens[s]}")
+
+
+@pytest.mark.parametrize("keys", [1, 2, 33, 129, 517, 1000])
+def test_decode_default_splits_and_large_scores(dev, keys):
+    """queries and keys of several times the usual size: one key takes most of the weight"""
+    from livecc_amd import ops
+    heads, kv_heads = 14, 2
+    kv = filled(dev, rand((1, kv_heads, keys, 128), dev, 1, 3.0), rand((1, kv_heads, keys, 128), dev, 2))
+    q = rand((1, heads * 128), dev, 3, 3.0)
+    kk, vv = values(kv, 0)
+    want, tol = U.attention(q.cpu().view(1, heads, 128), kk, vv, [keys - 1])
+    lens = i32([keys - 1], dev)
+    for nsplit in (0, ops.kv4_decode_splits([keys], kv_heads), 64):
+        got = ops.attn_decode4(q, kv, 0, i32([0], dev), lens, heads, nsplit)
+        U.assert_within(got, want.flatten(1), tol.flatten(1), f"nsplit {nsplit}")
+
+
+def test_decode_rows_without_keys_and_garbage_behind_the_length(dev):
+    """A length of -1 and slots out of range: zeros.  Bytes behind a stream's last key -- any codes, any scales, NaN's and those that overflow -- do not reach its result; a
+    length behind the arena counts as the arena's."""
+    from livecc_amd import ops
+    heads, kv_heads, L = 14, 2, 96
+    kv = filled(dev, rand((5, kv_heads, L, 128), dev, 1), rand((5, kv_heads, L, 128), dev, 2))
+    lens = [-1, 40, 95, 4000, -7]
+    clean = [values(kv, s) for s in range(5)]
+    kc, vc, ks, vs = kv._layer(1, 0)
+    ks.view(kv_heads, L, 4)[:, 41:] = 255
+    kc.view(kv_heads, L, 64)[:, 41:] = 0x77
+    scales = vs.view(kv_heads, L // 32, 4, 4, 8)
+    scales[:, 2] = 254
+    scales[:, 1, 2:] = 255                        # positions 48 ..
+    scales[:, 1, 1, :, 1:] = 253                  # positions 41 .. 47
+    q = rand((7, heads * 128), dev, 3)
+    slots = [0, 1, 2, 3, 4, -1, 5]
+    for nsplit in (1, 3):
+        got = ops.attn_decode4(q, kv, 0, i32(slots, dev), i32(lens, dev), heads, nsplit)
+        for i, s in enumerate(slots):
+            if s in (1, 2, 3):
+                want, tol = U.attention(q[i:i + 1].cpu().view(1, heads, 128), *clean[s], [min(lens[s], L - 1)])
+                U.assert_within(got[i], want[0].flatten(), tol[0].flatten(), f"row {i}")
+            else:
+                assert not got[i].any(), i
+
+
+def test_decode_nan_reaches_the_channels_and_heads_that_read_it(dev):
+    from livecc_amd import ops
+    heads, kv_heads, L = 4, 2, 64
+    k, v = rand((1, kv_heads, L, 128), dev, 1), rand((1, kv_heads, L, 128), dev, 2)
+    v[0, 1, 5, 40] = math.nan                     # group 1 of KV head 1
+    kv = filled(dev, k, v)
+    got = ops.attn_decode4(rand((1, heads * 128), dev, 3), kv, 0, i32([0], dev), i32([L - 1], dev), heads, 1).view(heads, 128)
+    nan = torch.isnan(got).cpu()
+    assert not nan[:2].any() and bool(nan[2:, 32:64].all()) and not nan[2:, :32].any() and not nan[2:, 64:].any()
+
+
+# ---- attention of chunks
+@pytest.mark.parametrize("heads,kv_heads", [(2, 1), (7, 1), (28, 4), (3, 3), (32, 2), (64, 8)])
+@pytest.mark.parametrize("segments", [[(0, 1, 0)], [(1, 5, 59)], [(0, 37, 0), (1, 3, 61), (2, 0, 5), (0, 2, 37)], [(2, 33, 30), (1, 64, 32)]])
+@pytest.mark.parametrize("nsplit", [1, 3])
+def test_chunk(dev, heads, kv_heads, segments, nsplit):
+    from livecc_amd import ops
+    L = 96
+    kv = filled(dev, rand((3, kv_heads, L, 128), dev, 1), rand((3, kv_heads, L, 128), dev, 2))
+    S = sum(n for _, n, _ in segments)
+    q = rand((S, heads * 128), dev, 3)
+    plan = ops.kv4_prefill_plan(segments, heads, kv_heads, dev, nsplit)
+    got = ops.attn_prefill4(q, kv, 0, plan, heads)
+    row = 0
+    for slot, n, past in segments:
+        if n == 0:
+            continue
+        kk, vv = values(kv, slot)
+        want, tol = U.attention(q[row:row + n].cpu().view(n, heads, 128), kk, vv, [past + r for r in range(n)])
+        U.assert_within(got[row:row + n], want.flatten(1), tol.flatten(1), f"{slot} {n} {past}")
+        row += n
+    if nsplit == 1:                               # the segments themselves are a plan; the default split count
+        U.assert_within(ops.attn_prefill4(q, kv, 0, segments, heads)[row - n:row], want.flatten(1), tol.flatten(1))
+
+
+@pytest.mark.parametrize("rows,past,heads,kv_heads", [(150, 1000, 7, 1), (2, 700, 28, 4), (300, 0, 12, 2)])
+def test_chunk_longer(dev, rows, past, heads, kv_heads):
+    from livecc_amd import ops
+    L = rows + past
+    kv = filled(dev, rand((1, kv_heads, L, 128), dev, 1, 2.0), rand((1, kv_heads, L, 128), dev, 2))
+    q = rand((rows, heads * 128), dev, 3, 1.5)
+    kk, vv = values(kv, 0)
+    got = ops.attn_prefill4(q, kv, 0, [(0, rows, past)], heads)
+    at = sorted({0, 1, rows // 2, rows - 2, rows - 1} & set(range(rows)))
+    want, tol = U.attention(q[at].cpu().view(len(at), heads, 128), kk, vv, [past + r for r in at])
+    U.assert_within(got[at], want.flatten(1), tol.flatten(1))
+    # every row against another order of the same sums
+    one = torch.cat([ops.attn_decode4(q[r:r + 1], kv, 0, i32([0], dev), i32([past + r], dev), heads, 1) for r in range(0, rows, 7)])
+    wide = (one.float() - got[::7].float()).abs()
+    top = kv.v_view(0, 0).float().abs().max()
+    assert bool((wide <= 2.0 ** -7 * top + 2.0 ** -7 * one.float().abs()).all())
+
+
+def test_chunk_rows_do_not_see_later_keys(dev):
+    """NaN keys and values of later rows of the same chunk, and garbage behind the stream's last key, reach no earlier row; the rows that see them are NaN where they are."""
+    from livecc_amd import ops
+    heads, kv_heads, L, past, n = 14, 2, 128, 50, 40
+    k, v = rand((1, kv_heads, L, 128), dev, 1), rand((1, kv_heads, L, 128), dev, 2)
+    ck, cv = k.clone(), v.clone()
+    v[0, 0, 70, 3] = math.nan                     # group 0 of KV head 0, seen from row 20 on
+    v[0, 1, 66, 127] = math.inf                   # group 3 of KV head 1, from row 16
+    k[0, 1, 80, 9] = math.nan                     # all of KV head 1, from row 30
+    clean, kv = filled(dev, ck, cv), filled(dev, k, v)
+    kc, vc, ks, vs = kv._layer(0, 0)
+    ks.view(kv_heads, L, 4)[:, 90:] = 255
+    vs.view(kv_heads, L // 32, 4, 4, 8)[:, 3] = 253
+    vs.view(kv_heads, L // 32, 4, 4, 8)[:, 2, 3, :, 2:] = 255     # positions 90 ..
+    q = rand((n, heads * 128), dev, 3)
+    kk, vv = values(clean, 0)
+    want, tol = U.attention(q.cpu().view(n, heads, 128), kk, vv, [past + r for r in range(n)])
+    want[20:, :7, :32] = math.nan
+    want[16:, 7:, 96:] = math.nan
+    want[30:, 7:] = math.nan
+    for nsplit in (1, 2):
+        got = ops.attn_prefill4(q, kv, 0, ops.kv4_prefill_plan([(0, n, past)], heads, kv_heads, dev, nsplit), heads)
+        U.assert_within(got, want.flatten(1), tol.flatten(1), f"nsplit {nsplit}")
+
+
+def test_chunk_of_a_slot_that_does_not_exist(dev):
+    from livecc_amd import ops
+    kv = filled(dev, rand((2, 1, 64, 128), dev, 1), rand((2, 1, 64, 128), dev, 2))
+    q = rand((9, 7 * 128), dev, 3)
+    for nsplit in (1, 2):
+        got = ops.attn_prefill4(q, kv, 0, ops.kv4_prefill_plan([(-1, 3, 0), (1, 3, 20), (2, 3, 4)], 7, 1, dev, nsplit), 7)
+        assert not got[:3].any() and not got[6:].any() and bool(got[3:6].any())
+
+
+# ---- the set together
+@pytest.mark.parametrize("heads,kv_heads", [(7, 1), (12, 2)])
+def test_a_stream_is_prefilled_and_decoded(dev, heads, kv_heads):
+    """Two streams: first turn, a second chunk, then single tokens, each appended and attended to as a layer does it; the reference works on the 64-bit definition from
+    the projections on."""
+    from livecc_amd import ops
+    lmax, layers, layer = 160, 2, 1
+    kv = ops.Kv4Arena(3, layers, kv_heads, lmax, dev)
+    qn, kn = rand((128,), dev, 11), rand((128,), dev, 12)
+    slots = (2, 0)
+    have = {s: (torch.zeros(kv_heads, lmax, 128, dtype=torch.float64), torch.zeros(kv_heads, lmax, 128, dtype=torch.float64), 0) for s in slots}
+    for turn, new in enumerate([(37, 50), (40, 3), (1, 1), (1, 1)]):
+        stream = [s for s, n in zip(slots, new) for _ in range(n)]
+        pos = [have[s][2] + r for s, n in zip(slots, new) for r in range(n)]
+        qkv = rand((len(stream), (heads + 2 * kv_heads) * 128), dev, 20 + turn)
+        cos, sin = tables(pos, dev)
+        decode = max(new) == 1
+        lens = i32([have.get(s, (0, 0, 0))[2] for s in range(3)], dev)
+        q = ops.qk_norm_rope_kv_append(qkv, cos, sin, i32(stream, dev), None if decode else i32(pos, dev), kv, layer, heads, q_norm=qn, k_norm=kn, kv_len=lens if decode else None)
+        if decode:
+            got = ops.attn_decode4(q, kv, layer, i32(stream, dev), lens, heads, 2)
+        else:
+            got = ops.attn_prefill4(q, kv, layer, [(s, n, have[s][2]) for s, n in zip(slots, new)], heads)
+        x = qkv.cpu().view(len(stream), heads + 2 * kv_heads, 128)
+        wq = U.norm_rope(x[:, :heads], qn.cpu(), cos.cpu(), sin.cpu())
+        wk = U.quantise(U.norm_rope(x[:, heads:heads + kv_heads], kn.cpu(), cos.cpu(), sin.cpu()))[2]
+        wv = U.quantise(x[:, heads + kv_heads:])[2]
+        row = 0
+        for s, n in zip(slots, new):
+            k, v, p = have[s]
+            k[:, p:p + n], v[:, p:p + n] = wk[row:row + n].transpose(0, 1), wv[row:row + n].transpose(0, 1)
+            want, tol = U.attention(wq[row:row + n], k, v, [p + r for r in range(n)])
+            U.assert_within(got[row:row + n], want.flatten(1), tol.flatten(1), f"turn {turn} slot {s}")
+            have[s] = (k, v, p + n)
+            row += n
+
+
+def test_a_captured_step_is_replayed(dev):
+    """append + decode attention + chunk attention in one graph: replays follow what the buffers then hold, with eager work in between"""
+    from livecc_amd import ops
+    heads, kv_heads, lmax = 12, 2, 640
+    kv, kv2 = ops.Kv4Arena(2, 1, kv_heads, lmax, dev), ops.Kv4Arena(2, 1, kv_heads, lmax, dev)
+    qn, kn = rand((128,), dev, 11), rand((128,), dev, 12)
+    qkv, st, lens = rand((2, 16 * 128), dev, 1), i32([0, 1], dev), i32([500, 77], dev)
+    cos, sin = tables([500, 77], dev)
+    qc = rand((60, heads * 128), dev, 2)
+    plan = ops.kv4_prefill_plan([(0, 40, 440), (1, 20, 50)], heads, kv_heads, dev, 2)
+
+    def step(c):
+        q = ops.qk_norm_rope_kv_append(qkv, cos, sin, st, None, c, 0, heads, q_norm=qn, k_norm=kn, kv_len=lens)
+        return q, ops.attn_decode4(q, c, 0, st, lens, heads, 3), ops.attn_prefill4(qc, c, 0, plan, heads)
+    for c in (kv, kv2):
+        hist = rand((2 * lmax, 4 * 128), dev, 3)
+        one = torch.ones(2 * lmax, 64, dtype=torch.bfloat16, device=dev)
+        ops.qk_norm_rope_kv_append(hist, one, one * 0, torch.arange(2, dtype=torch.int32, device=dev).repeat_interleave(lmax),
+                                   torch.arange(lmax, dtype=torch.int32, device=dev).repeat(2), c, 0, 0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(kv2)
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step(kv)
+    for i in range(4):
+        qkv.copy_(rand((2, 16 * 128), dev, 30 + i))
+        lens.copy_(i32([500 + i, 77 - i], dev))
+        g.replay()
+        want = step(kv2)
+        torch.cuda.synchronize()
+        for a, b in zip(out, want):
+            assert torch.equal(a, b), i
+        assert torch.equal(kv.buf, kv2.buf)
+
+
+def test_on_a_stream_of_its_own_and_two_at_once(dev):
+    from livecc_amd import ops
+    heads, kv_heads, L = 28, 4, 700
+    kv = filled(dev, rand((2, kv_heads, L, 128), dev, 1), rand((2, kv_heads, L, 128), dev, 2))
+    q = [rand((2, heads * 128), dev, 3 + i) for i in range(2)]
+    slots, lens = i32([0, 1], dev), i32([L - 1, 333], dev)
+    want = [ops.attn_decode4(x, kv, 0, slots, lens, heads, 4) for x in q]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(ops.attn_decode4(q[i], kv, 0, slots, lens, heads, 4))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for x in got[i]:
+            assert torch.equal(x, want[i])
+
+
+def test_offsets_beyond_32_bits(dev):
+    """the last layer of a slot of more than 4 GiB"""
+    from livecc_amd import ops
+    heads, kv_heads, lmax, layers = 16, 8, 32768, 124
+    kv = ops.Kv4Arena(1, layers, kv_heads, lmax, dev)
+    assert kv.per_slot > 1 << 32
+    last, n = layers - 1, 70
+    pos = list(range(lmax - n, lmax))
+    qkv = rand((n, 32 * 128), dev, 1)
+    cos, sin = tables(pos, dev)
+    st = i32([0] * n, dev)
+    q = ops.qk_norm_rope_kv_append(qkv, cos, sin, st, i32(pos, dev), kv, last, heads)
+    k, v = ops.kv4_read(kv, last, st, i32(pos, dev))
+    x = qkv.cpu().view(n, 32, 128)
+    assert torch.equal(v.double().cpu(), U.quantise(x[:, 24:])[2])
+    assert torch.equal(k.double().cpu(), U.quantise(U.norm_rope(x[:, 16:24], None, cos.cpu(), sin.cpu()))[2])
+    kk, vv = values(kv, 0, last)
+    assert torch.equal(kk[:, -n:].transpose(0, 1), k.double().cpu())
+    want, tol = U.attention(q[-1:].cpu().view(1, heads, 128), kk, vv, [lmax - 1])
+    U.assert_within(ops.attn_decode4(q[-1:].contiguous(), kv, last, i32([0], dev), i32([lmax - 1], dev), heads), want.flatten(1), tol.flatten(1))
+    U.assert_within(ops.attn_prefill4(q[-1:].contiguous(), kv, last, [(0, 1, lmax - 1)], heads), want.flatten(1), tol.flatten(1))
+
+
+@pytest.mark.parametrize("through", ["torch", "ctypes"])
+def test_refusals(dev, through, monkeypatch):
+    from livecc_amd import _lib, ops, torch_ops
+    if through == "ctypes":
+        monkeypatch.setattr(torch_ops, "op", lambda name: None)
+    heads, kv_heads, S = 4, 2, 3
+    kv, kv16 = ops.Kv4Arena(2, 1, kv_heads, 64, dev), ops.KvArena(2, 1, kv_heads, 64, dev)
+    qkv, st, pos = rand((S, 8 * 128), dev, 1), i32([0, 1, 1], dev), i32([0, 0, 1], dev)
+    cos, sin = tables([0, 0, 1], dev)
+    w = rand((128,), dev, 2)
+    err = (_lib.LccError, ValueError, TypeError)
+    for bad in (lambda: ops.qk_norm_rope_kv_append(None, cos, sin, st, pos, kv, 0, heads),
+                lambda: ops.qk_norm_rope_kv_append(qkv.float(), cos, sin, st, pos, kv, 0, heads),
+                lambda: ops.qk_norm_rope_kv_append(qkv[:, :-128].contiguous(), cos, sin, st, pos, kv, 0, heads),
+                lambda: ops.qk_norm_rope_kv_append(qkv, cos, sin[:2], st, pos, kv, 0, heads),
+                lambda: ops.qk_norm_rope_kv_append(qkv, cos, sin, st[:2], pos, kv, 0, heads),
+                lambda: ops.qk_norm_rope_kv_append(qkv, cos, sin, st, None, kv, 0, heads),
+                lambda: ops.qk_norm_rope_kv_append(qkv, cos, sin, st, None, kv, 0, heads, kv_len=st[:1]),
+                lambda: ops.qk_norm_rope_kv_append(qkv, cos, sin, st.long(), pos, kv, 0, heads),
+                lambda: ops.qk_norm_rope_kv_append(qkv, cos, sin, st, pos, kv, 1, heads),
+                lambda: ops.qk_norm_rope_kv_append(qkv, cos, sin, st, pos, kv, 0, heads, q_norm=w[:64]),
+                lambda: ops.qk_norm_rope_kv_append(qkv, cos, sin, st, pos, kv, 0, heads, q_norm=w, eps=0.0),
+                lambda: ops.qk_norm_rope_kv_append(qkv, cos, sin, st, pos, kv, 0, heads, q_norm=w, eps=float("nan")),
+                lambda: ops.qk_norm_rope_kv_append(qkv, cos, sin, st, pos, kv, 0, heads, bias=rand((8 * 128,), dev, 1)),
+                lambda: ops.qk_norm_rope_kv_append(None, cos, sin, st, pos, kv, 0, heads, partial=torch.zeros(9, S, 8 * 128, device=dev)),
+                lambda: ops.kv4_read(kv, 0, st, pos[:2]), lambda: ops.kv4_read(kv16, 0, st, pos), lambda: ops.kv4_read(kv, -1, st, pos),
+                lambda: ops.attn_decode4(qkv[:, :512].contiguous(), kv16, 0, st, pos, heads),
+                lambda: ops.attn_decode4(qkv[:, :512], kv, 0, st, pos, heads),
+                lambda: ops.attn_decode4(qkv[:, :512].contiguous(), kv, 0, st[:2], pos, heads),
+                lambda: ops.attn_decode4(qkv[:, :512].contiguous(), kv, 0, st, pos[:1], heads),
+                lambda: ops.attn_decode4(qkv[:, :512].contiguous(), kv, 0, st, pos, heads, 65),
+                lambda: ops.attn_decode4(qkv[:, :384].contiguous(), kv, 0, st, pos, 3),
+                lambda: ops.attn_decode4(rand((S, 34 * 128), dev, 1), kv, 0, st, pos, 34),
+                lambda: ops.attn_prefill4(qkv[:, :512].contiguous(), kv, 0, [(0, 2, 0)], heads),
+                lambda: ops.attn_prefill4(qkv[:, :512].contiguous(), kv, 0, [(0, 3, 62)], heads),
+                lambda: ops.attn_prefill4(qkv[:, :512].contiguous(), kv, 0, ops.kv4_prefill_plan([(0, 3, 0)], heads, kv_heads, dev, 33), heads),
+                lambda: ops.attn_prefill4(qkv[:, :512].contiguous(), kv, 0, ops.kv4_prefill_plan([(0, 3, 0)], 8, kv_heads, dev), heads)):
+        with pytest.raises(err):
+            bad()
+    assert not kv.buf.any()
+    # and calls of nothing
+    z = qkv[:0]
+    assert ops.qk_norm_rope_kv_append(z, cos[:0], sin[:0], st[:0], pos[:0], kv, 0, heads).shape == (0, 512)
+    assert ops.attn_decode4(z[:, :512].contiguous(), kv, 0, st[:0], pos, heads).shape == (0, 512)
+    assert ops.attn_prefill4(z[:, :512].contiguous(), kv, 0, [], heads).shape == (0, 512)
+    assert ops.kv4_read(kv, 0, st[:0], pos[:0])[0].shape == (0, kv_heads, 128)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_through_the_c_abi_as_through_torch(dev, bits, monkeypatch):
+    from livecc_amd import ops, torch_ops
+    heads, kv_heads, S = 7, 1, 40
+    qkv, cs = rand((S, 9 * 128), dev, 1), tables(range(S), dev)
+    st, pos, w = i32([0] * S, dev), i32(list(range(S)), dev), rand((128,), dev, 2)
+
+    def go():
+        kv = (ops.Kv4Arena if bits == 4 else ops.KvArena)(1, 1, kv_heads, 64, dev)
+        q = ops.qk_norm_rope_kv_append(qkv, *cs, st, pos, kv, 0, heads, q_norm=w, k_norm=w)
+        if bits == 16:
+            return q, kv.buf
+        return (q, kv.buf, *ops.kv4_read(kv, 0, st, pos), ops.attn_decode4(q[:2].contiguous(), kv, 0, st[:2], i32([S - 1], dev), heads, 2),
+                ops.attn_prefill4(q, kv, 0, ops.kv4_prefill_plan([(0, S, 0)], heads, kv_heads, dev, 2), heads))
+    n = sum(torch_ops.CALLS[k] for k in ("qk_norm_rope_kv_append", "attn_decode4", "attn_prefill4", "kv4_read"))
+    a = go()
+    assert sum(torch_ops.CALLS[k] for k in ("qk_norm_rope_kv_append", "attn_decode4", "attn_prefill4", "kv4_read")) == n + (4 if bits == 4 else 1)
+    monkeypatch.setattr(torch_ops, "op", lambda name: None)
+    for x, y in zip(a, go()):
+        assert torch.equal(x, y)
