@@ -15,12 +15,21 @@
 //     values of a byte are of one token (tokens never share a byte: appends need no read-modify-write, two streams' appends no order) and one scale, and
 //     a lane's 32 bytes (g, i) are its operand of the eight 16x16x32 products over the block.
 //   K scales [head][position][4], V scales [head][position / 32][g 4][t 4][e 8].
+#include <algorithm>
+#include <type_traits>
+#include <utility>
+
 #include "common.h"
 #include "kernels.h"
 
 namespace lcc {
 
 typedef __attribute__((ext_vector_type(16))) float f32x16;
+
+template <class F, int... I>
+LCC_DEVICE void unrolled_of(F&& f, std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>{}), ...); }
+template <int N, class F>
+LCC_DEVICE void unrolled(F&& f) { unrolled_of(f, std::make_integer_sequence<int, N>{}); }      // f(0) .. f(N - 1), the index a constant
 
 LCC_DEVICE f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 LCC_DEVICE int swap23(int i) { return (i & ~12) | ((i & 4) << 1) | ((i & 8) >> 1); }
@@ -30,6 +39,15 @@ LCC_DEVICE float xor32_max(float x) {
 }
 LCC_DEVICE float xor32_sum(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+LCC_DEVICE float xor16_max(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __builtin_fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+LCC_DEVICE float xor16_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
@@ -273,26 +291,31 @@ int kv4_read(const Kv4Args& a, const int32_t* tok_stream, const int32_t* tok_pos
 // channels of step s are 8 s .. 8 s + 7 of each group, for Q alike.  Rows of the two key tiles are dealt so that a lane's eight scores are of the keys
 // 8 g .. 8 g + 7, which are the slots of its P operand: O^T += V^T P^T takes the probabilities from the softmax' registers and V's bytes as they lie.
 // ------------------------------------------------------------------------------------------------------------------------------
+constexpr float KV4_SLACK = 8.f;
 struct Kv4Tile { u32x4 k[2], v[2], s[2]; unsigned ks[2]; };       // what a wave loads of a 32-key block: codes of two key tiles, of V, V's scales, K's
-LCC_DEVICE void kv4_load(Kv4Tile& t, const uint8_t* kc, const uint8_t* vc, const uint8_t* ks, const uint8_t* vs, int blk, int li, int g) {
-  const int key = 8 * (li >> 2) + (li & 3);
+struct Kv4Head { const uint8_t *kc, *vc, *ks, *vs; };              // a head's regions, wave-uniform: a lane's part of the addresses is 32 bits that never change
+LCC_DEVICE void kv4_load_k(Kv4Tile& t, const Kv4Head& h, int blk, unsigned key, unsigned g) {
+  const uint8_t *kc = h.kc + (size_t)blk * 2048, *ks = h.ks + (size_t)blk * 128;
 #pragma unroll
-  for (int T = 0; T < 2; ++T) {
-    t.k[T] = ld16(kc + ((size_t)blk * 32 + key + 4 * T) * 64 + g * 16);
-    t.ks[T] = ks[((size_t)blk * 32 + key + 4 * T) * 4 + g];
+  for (unsigned T = 0; T < 2; ++T) {
+    t.k[T] = ld16(kc + (key * 64 + g * 16 + T * 256));
+    t.ks[T] = ks[key * 4 + g + T * 16];
   }
-  const uint8_t* v = vc + (size_t)blk * 2048 + g * 512 + li * 32;
-  const uint8_t* s = vs + (size_t)blk * 128 + g * 32;
-  t.v[0] = ld16(v); t.v[1] = ld16(v + 16); t.s[0] = ld16(s); t.s[1] = ld16(s + 16);
+}
+LCC_DEVICE void kv4_load_v(Kv4Tile& t, const Kv4Head& h, int blk, unsigned li, unsigned g) {
+  const uint8_t *vc = h.vc + (size_t)blk * 2048, *vs = h.vs + (size_t)blk * 128;
+  t.v[0] = ld16(vc + (g * 512 + li * 32)); t.v[1] = ld16(vc + (g * 512 + li * 32 + 16));
+  t.s[0] = ld16(vs + g * 32); t.s[1] = ld16(vs + (g * 32 + 16));
 }
 
 template <int NW>
-__global__ __launch_bounds__(NW * 64, 2) void attn_decode_kv4_kernel(Kv4Args a, const bf16_t* __restrict__ q, const int32_t* __restrict__ slots,
+__global__ __launch_bounds__(NW * 64, 4) void attn_decode_kv4_kernel(Kv4Args a, const bf16_t* __restrict__ q, const int32_t* __restrict__ slots,
                                                                      const int32_t* __restrict__ kv_len, int n_q_heads, int nsplit,
                                                                      float* __restrict__ ws_o, float* __restrict__ ws_ml, bf16_t* __restrict__ out, float scale_log2e) {
-  __shared__ float mo[NW][16][132];
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+  float (*mo)[16][132] = reinterpret_cast<float (*)[16][132]>(lds);
   __shared__ float mm[NW][16], ml[NW][16];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, g = lane >> 4;
   const int split = blockIdx.x, hk = blockIdx.y, b = blockIdx.z, G = n_q_heads / a.n_kv_heads;
   const int slot = slots[b];
   const bool live = slot >= 0 && slot < a.n_slots;
@@ -307,15 +330,19 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_decode_kv4_kernel(Kv4Args a, 
   if (blk < b1) {
     const Kv4Layout lay{a.n_kv_heads, a.lmax};
     const uint8_t* base = (const uint8_t*)a.kv_base[slot] + (size_t)a.layer * lay.layer_bytes();
-    const uint8_t *kc = base + lay.k_codes(hk), *vc = base + lay.v_codes(hk), *ks = base + lay.k_scales(hk), *vs = base + lay.v_scales(hk);
+    const Kv4Head head{base + lay.k_codes(hk), base + lay.v_codes(hk), base + lay.k_scales(hk), base + lay.v_scales(hk)};
+    const unsigned key = 8 * (li >> 2) + (li & 3);
     u32x4 qf[4];
     const bf16_t* qp = q + ((size_t)b * n_q_heads + hk * G + min(li, G - 1)) * 128 + g * 32;
 #pragma unroll
     for (int s = 0; s < 4; ++s) qf[s] = ld16(qp + 8 * s);
-    Kv4Tile cur, nxt;
-    kv4_load(cur, kc, vc, ks, vs, blk, li, g);
+    Kv4Tile cur;
+    kv4_load_k(cur, head, blk, key, g);
+    asm volatile("" ::: "memory");             // in the loop's order, so that its waits hold for the first turn, too
+    kv4_load_v(cur, head, blk, li, g);
+    asm volatile("" ::: "memory");
     for (; blk < b1; blk += NW) {
-      if (blk + NW < b1) kv4_load(nxt, kc, vc, ks, vs, blk + NW, li, g);
+      const int nb = blk + NW < b1 ? blk + NW : blk;                        // behind the last: the same again, so that a wait can count what is in flight
       f32x4 sc[2];
 #pragma unroll
       for (int T = 0; T < 2; ++T) {
@@ -323,6 +350,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_decode_kv4_kernel(Kv4Args a, 
 #pragma unroll
         for (int s = 0; s < 4; ++s) sc[T] = mfma16(as_bf16x8(fp4_word(cur.k[T][s], cur.ks[T] << 23)), as_bf16x8(qf[s]), sc[T]);
       }
+      kv4_load_k(cur, head, nb, key, g);                                    // into the registers that the products have left
       const int left = n - blk * 32 - 8 * g;                                // keys of this lane's octet that exist
       if (n - blk * 32 < 32) {                                              // the last block: scores of no key to -inf, V there to zero (0 * NaN)
 #pragma unroll
@@ -335,11 +363,9 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_decode_kv4_kernel(Kv4Args a, 
       }
       float top = __builtin_fmaxf(__builtin_fmaxf(__builtin_fmaxf(sc[0][0], sc[0][1]), __builtin_fmaxf(sc[0][2], sc[0][3])),
                                   __builtin_fmaxf(__builtin_fmaxf(sc[1][0], sc[1][1]), __builtin_fmaxf(sc[1][2], sc[1][3])));
-      top = __builtin_fmaxf(top, __shfl_xor(top, 16, 64));
-      top = xor32_max(top);
-      const float mn = __builtin_fmaxf(m, top * scale_log2e), mu = mn == -INFINITY ? 0.f : mn;
-      if (__any(mn > m)) {
-        const float f = __builtin_amdgcn_exp2f(m - mu);
+      top = xor32_max(xor16_max(top)) * scale_log2e;
+      if (__any(top > m + KV4_SLACK)) {
+        const float mn = __builtin_fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - mn);
         l *= f;
 #pragma unroll
         for (int t = 0; t < 8; ++t) o[t] *= f;
@@ -347,19 +373,24 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_decode_kv4_kernel(Kv4Args a, 
       }
       float p[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) { p[e] = __builtin_amdgcn_exp2f(fmaf(sc[e >> 2][e & 3], scale_log2e, -mu)); l += p[e]; }
-      const bf16x8 pf = as_bf16x8((u32x4){pack2(p[0], p[1]), pack2(p[2], p[3]), pack2(p[4], p[5]), pack2(p[6], p[7])});
+      for (int e = 0; e < 8; ++e) { p[e] = __builtin_amdgcn_exp2f(fmaf(sc[e >> 2][e & 3], scale_log2e, -m)); l += p[e]; }
+      // A converted byte is a pair (channel i, channel 16 + i) of one key, two slots of the operand: against (p, 0) it is channel i's product, against (0, p) the other's.
+      u32x4 pl[2], ph[2];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        u32x4 lo, hi;
-        fp4_octet((u32x2){cur.v[t >> 1][2 * (t & 1)], cur.v[t >> 1][2 * (t & 1) + 1]}, (u32x2){cur.s[t >> 1][2 * (t & 1)], cur.s[t >> 1][2 * (t & 1) + 1]}, lo, hi);
-        o[2 * t] = mfma16(as_bf16x8(lo), pf, o[2 * t]);
-        o[2 * t + 1] = mfma16(as_bf16x8(hi), pf, o[2 * t + 1]);
-      }
-      cur = nxt;
+      for (int e = 0; e < 8; ++e) { pl[e >> 2][e & 3] = pack2(p[e], 0.f); ph[e >> 2][e & 3] = pl[e >> 2][e & 3] << 16; }
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+          const unsigned w = cur.v[t >> 1][2 * (t & 1) + z], sw = cur.s[t >> 1][2 * (t & 1) + z];
+          const bf16x8 v = as_bf16x8((u32x4){fp4_pair<0>(w, scale_of<0>(sw)), fp4_pair<1>(w, scale_of<1>(sw)), fp4_pair<2>(w, scale_of<2>(sw)), fp4_pair<3>(w, scale_of<3>(sw))});
+          o[2 * t] = mfma16(v, as_bf16x8(pl[z]), o[2 * t]);
+          o[2 * t + 1] = mfma16(v, as_bf16x8(ph[z]), o[2 * t + 1]);
+        }
+      kv4_load_v(cur, head, nb, li, g);
+      asm volatile("" ::: "memory");           // hipcc would move the loads to the head of the next turn, in front of their wait
     }
-    l += __shfl_xor(l, 16, 64);
-    l = xor32_sum(l);
+    l = xor32_sum(xor16_sum(l));
   }
   // the waves' parts, joined in LDS: column li, channels 16 t + 4 g .. + 3
 #pragma unroll
@@ -390,38 +421,58 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_decode_kv4_kernel(Kv4Args a, 
   }
 }
 
-// Joins the key splits of a (row, head): sums weighted by 2^(m - max), one rounding.
-__global__ __launch_bounds__(256) void kv4_combine_kernel(const float* __restrict__ ws_o, const float* __restrict__ ws_ml, bf16_t* __restrict__ out, int nsplit) {
-  __shared__ f32x4 so[8][32];
-  __shared__ float sl[8];
-  const size_t row = (size_t)blockIdx.x;
-  const int grp = threadIdx.x >> 5, c = threadIdx.x & 31;
-  float M = -INFINITY;
-  for (int s = 0; s < nsplit; ++s) M = __builtin_fmaxf(M, ws_ml[(row * nsplit + s) * 2]);
-  const float mu = M == -INFINITY ? 0.f : M;
-  f32x4 acc = (f32x4){0.f, 0.f, 0.f, 0.f};
-  float L = 0.f;
-  for (int s = grp; s < nsplit; s += 8) {
-    const float f = __builtin_amdgcn_exp2f(ws_ml[(row * nsplit + s) * 2] - mu);
-    L += f * ws_ml[(row * nsplit + s) * 2 + 1];
-    acc += f * *reinterpret_cast<const f32x4*>(ws_o + (row * nsplit + s) * 128 + c * 4);
+// Joins the key splits of a (row, head): sums weighted by 2^(m - max), one rounding.  A half-wave reads a split's 128 channels at a time; W waves share a (row, head).
+template <int W>
+__global__ __launch_bounds__(256) void kv4_combine_kernel(const float* __restrict__ ws_o, const float* __restrict__ ws_ml, bf16_t* __restrict__ out, int64_t n, int nsplit) {
+  __shared__ f32x4 so[W][32];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, c = lane & 31;
+  const int64_t row = W == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
+  if (row >= n) return;                                                     // whole waves, and W > 1: none
+  const float* ml = ws_ml + (size_t)row * nsplit * 2;
+  const float* o = ws_o + (size_t)row * nsplit * 128 + c * 4;
+  constexpr int N = W == 1 ? 4 : 8;                                          // a half-wave's share of 8 or 64 splits, all in flight before the weights are formed
+  const int s0 = wave * (W == 1 ? 0 : 2) + half;
+  f32x4 v[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int s = s0 + 2 * W * i;
+    v[i] = s < nsplit ? *reinterpret_cast<const f32x4*>(o + (size_t)s * 128) : (f32x4){0.f, 0.f, 0.f, 0.f};
   }
-  so[grp][c] = acc;
-  if (c == 0) sl[grp] = L;
-  __syncthreads();
-  if (grp != 0) return;
-  for (int i = 1; i < 8; ++i) { acc += so[i][c]; L += sl[i]; }
+  const float m = lane < nsplit ? ml[lane * 2] : -INFINITY, l = lane < nsplit ? ml[lane * 2 + 1] : 0.f;
+  const float M = wave_max(m), w = __builtin_amdgcn_exp2f(m - (M == -INFINITY ? 0.f : M));
+  const float L = wave_sum(w * l);
+  f32x4 acc = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int s = s0 + 2 * W * i;
+    const float f = __shfl(w, s & 63, 64);
+    if (s < nsplit) acc += f * v[i];
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) acc[e] = xor32_sum(acc[e]);
+  if (W > 1) {
+    if (half == 0) so[wave][c] = acc;
+    __syncthreads();
+    if (wave != 0) return;
+    acc = so[0][c];
+#pragma unroll
+    for (int i = 1; i < W; ++i) acc += so[i][c];
+  }
   const float r = L == 0.f ? 0.f : 1.f / L;
-  st8(out + row * 128 + c * 4, (u32x2){pack2(acc[0] * r, acc[1] * r), pack2(acc[2] * r, acc[3] * r)});
+  if (half == 0) st8(out + (size_t)row * 128 + c * 4, (u32x2){pack2(acc[0] * r, acc[1] * r), pack2(acc[2] * r, acc[3] * r)});
+}
+static void kv4_combine(const float* ws_o, const float* ws_ml, bf16_t* out, int64_t n, int nsplit, hipStream_t st) {
+  if (nsplit <= 8) kv4_combine_kernel<1><<<dim3((unsigned)((n + 3) / 4)), dim3(256), 0, st>>>(ws_o, ws_ml, out, n, nsplit);
+  else kv4_combine_kernel<4><<<dim3((unsigned)n), dim3(256), 0, st>>>(ws_o, ws_ml, out, n, nsplit);
 }
 
 int kv4_decode_splits(const int32_t* n_keys, int n, int n_kv_heads) {
   long most = 1;
   for (int i = 0; i < n; ++i) most = n_keys[i] > most ? n_keys[i] : most;
   const long blocks = (most + 31) / 32, base = (long)(n > 0 ? n : 1) * n_kv_heads;
-  long k = (512 + base - 1) / base;
-  if (k > (blocks + 7) / 8) k = (blocks + 7) / 8;
-  return (int)(k < 1 ? 1 : k > 64 ? 64 : k);
+  if (blocks <= 32) return 1;
+  const long k = std::min((256 + base - 1) / base, std::min(blocks / 4, 64L));
+  return (int)std::max(k, 1L);
 }
 
 int attn_decode_kv4(const Kv4Args& a, const bf16_t* q, const int32_t* slots, const int32_t* kv_len, int rows, int n_q_heads, int nsplit, float* ws_o, float* ws_ml,
@@ -431,8 +482,14 @@ int attn_decode_kv4(const Kv4Args& a, const bf16_t* q, const int32_t* slots, con
     return LCC_ERR_SHAPE;
   if (nsplit > 1 && (ws_o == nullptr || ws_ml == nullptr)) return LCC_ERR_ARG;
   if (rows == 0) return 0;
-  attn_decode_kv4_kernel<4><<<dim3(nsplit, a.n_kv_heads, rows), dim3(256), 0, st>>>(a, q, slots, kv_len, n_q_heads, nsplit, ws_o, ws_ml, out, 1.4426950408889634f / sqrtf(128.f));
-  if (nsplit > 1) kv4_combine_kernel<<<dim3((unsigned)(rows * n_q_heads)), dim3(256), 0, st>>>(ws_o, ws_ml, out, nsplit);
+  static DeviceOnce once;
+  constexpr int part = 16 * 132 * 4;                                        // LDS of a wave's result
+  if (once.first()) (void)hipFuncSetAttribute((const void*)attn_decode_kv4_kernel<8>, hipFuncAttributeMaxDynamicSharedMemorySize, 8 * part);
+  const dim3 grid(nsplit, a.n_kv_heads, rows);
+  const float scale = 1.4426950408889634f / sqrtf(128.f);
+  if (nsplit == 1) attn_decode_kv4_kernel<8><<<grid, dim3(512), 8 * part, st>>>(a, q, slots, kv_len, n_q_heads, nsplit, ws_o, ws_ml, out, scale);
+  else attn_decode_kv4_kernel<4><<<grid, dim3(256), 4 * part, st>>>(a, q, slots, kv_len, n_q_heads, nsplit, ws_o, ws_ml, out, scale);
+  if (nsplit > 1) kv4_combine(ws_o, ws_ml, out, (int64_t)rows * n_q_heads, nsplit, st);
   return 0;
 }
 
@@ -442,14 +499,16 @@ int attn_decode_kv4(const Kv4Args& a, const bf16_t* q, const int32_t* slots, con
 // O^T += V^T P^T on 32x32x16, K's rows read in the order (bits 2 and 3 swapped) that leaves a lane the scores of the keys its P operand wants.
 // ------------------------------------------------------------------------------------------------------------------------------
 constexpr int KV4_STAGE = 64, KV4_KB = KV4_STAGE * 256, KV4_VB = 128 * KV4_STAGE * 2, KV4_LDS = 2 * (KV4_KB + KV4_VB);
-struct Kv4Stage { u32x2 k, v, s; unsigned ks; };
+template <int U> struct Kv4Stage { u32x2 k[U], v[U], s[U]; unsigned ks[U]; };
 
-__global__ __launch_bounds__(512, 2) void attn_prefill_kv4_kernel(Kv4Args a, const bf16_t* __restrict__ q, bf16_t* __restrict__ out, const int32_t* __restrict__ tile_stream,
-                                                                  const int32_t* __restrict__ tile_q0, const int32_t* __restrict__ tile_nq,
-                                                                  const int32_t* __restrict__ tile_pos0, int n_q_heads, int tile_rows, int nsplit, int n_rows,
-                                                                  float* __restrict__ ws_o, float* __restrict__ ws_ml, float scale_log2e) {
+template <int NW>
+__global__ __launch_bounds__(NW * 64, 2) void attn_prefill_kv4_kernel(Kv4Args a, const bf16_t* __restrict__ q, bf16_t* __restrict__ out, const int32_t* __restrict__ tile_stream,
+                                                                      const int32_t* __restrict__ tile_q0, const int32_t* __restrict__ tile_nq,
+                                                                      const int32_t* __restrict__ tile_pos0, int n_q_heads, int tile_rows, int nsplit, int n_rows,
+                                                                      float* __restrict__ ws_o, float* __restrict__ ws_ml, float scale_log2e) {
+  constexpr int U = 8 / NW;                                                 // units of 8 bytes of K and of V that a thread stages
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
-  __shared__ unsigned long long bad[3][4];                                  // keys of a stage, by group, whose V is NaN (stages with masked scores)
+  __shared__ unsigned long long bad[4][4];                                  // keys of a stage, by group, whose V is NaN (stages with masked scores)
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, hh = lane >> 5, G = n_q_heads / a.n_kv_heads;
   const int hk = blockIdx.x, tile = blockIdx.y, split = blockIdx.z;
   const int slot = tile_stream[tile], q0 = tile_q0[tile], pos0 = min(tile_pos0[tile], a.lmax);
@@ -461,7 +520,6 @@ __global__ __launch_bounds__(512, 2) void attn_prefill_kv4_kernel(Kv4Args a, con
   const int c = wave * 32 + col, r = c / G, h = c - r * G;
   const bool valid = r < nq;
   const int lim = live ? pos0 + min(r, nq - 1) : -1;                        // last key this column sees
-  const bool active = wave * 32 < nq * G;                                   // wave-uniform
 
   u32x4 qf[8];
   const bf16_t* qp = q + ((size_t)(q0 + min(r, nq - 1)) * n_q_heads + hk * G + h) * 128 + hh * 8;
@@ -478,111 +536,183 @@ __global__ __launch_bounds__(512, 2) void attn_prefill_kv4_kernel(Kv4Args a, con
     const Kv4Layout lay{a.n_kv_heads, a.lmax};
     const uint8_t* base = (const uint8_t*)a.kv_base[slot] + (size_t)a.layer * lay.layer_bytes();
     const uint8_t *kc = base + lay.k_codes(hk), *vc = base + lay.v_codes(hk), *ksc = base + lay.k_scales(hk), *vsc = base + lay.v_scales(hk);
-    const int t = threadIdx.x, key = t >> 3, part = t & 7, vblk = t >> 8, vg = (t >> 6) & 3, vi = (t >> 2) & 15, vt = t & 3;
-    auto fetch = [&](Kv4Stage& x, int st) {
-      x.k = x.v = x.s = (u32x2){0u, 0u}; x.ks = 0u;
-      if (st * KV4_STAGE + key < a.lmax) {
-        x.k = ld8(kc + ((size_t)st * KV4_STAGE + key) * 64 + part * 8);
-        x.ks = ksc[((size_t)st * KV4_STAGE + key) * 4 + (part >> 1)];
+    const int t = threadIdx.x, last_blk = a.lmax / 32 - 1;
+    // Unit u of a thread: eight bytes of K (16 channels of a key) and of V (channels i, 16 + i of an octet of keys), number t + 64 NW u of the stage's two blocks of 256;
+    // the block is the same for a wave.  Behind the arena: its last block again (masked).
+    auto block_of = [&](int st, int u) { return (size_t)min(st * 2 + ((wave + u * NW) >> 2), last_blk); };
+    const unsigned unit = t & 255, s_off = ((t >> 6) & 3) * 32 + (t & 3) * 8;
+    auto fetch_k = [&](Kv4Stage<U>& x, int st) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        x.k[u] = ld8(kc + block_of(st, u) * 2048 + unit * 8);
+        x.ks[u] = (ksc + block_of(st, u) * 128)[unit >> 1];
       }
-      if (st * KV4_STAGE + vblk * 32 < a.lmax) {
-        x.v = ld8(vc + ((size_t)st * 2 + vblk) * 2048 + (t & 255) * 8);
-        x.s = ld8(vsc + ((size_t)st * 2 + vblk) * 128 + vg * 32 + vt * 8);
+    };
+    auto fetch_v = [&](Kv4Stage<U>& x, int st) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        x.v[u] = ld8(vc + block_of(st, u) * 2048 + unit * 8);
+        x.s[u] = ld8(vsc + block_of(st, u) * 128 + s_off);
       }
     };
     auto masked = [&](int st) { return st * KV4_STAGE + KV4_STAGE - 1 > pos0; };          // some row does not see all of the stage
-    auto stage = [&](Kv4Stage& x, int st) {
-      unsigned char* kb = lds + (st & 1) * (KV4_KB + KV4_VB);
-      unsigned char* vb = kb + KV4_KB;
-      if (masked(st)) {
-        // what a row does not see must not reach it through 0 * NaN: values behind the last key are zeros, and NaN values are zeros here and put into
-        // the rows that see them behind the product
-        const int k0 = st * KV4_STAGE + vblk * 32 + vg * 8;
+    const bool k_swap = (t & 4) != 0;
+    const unsigned kw_off = (t >> 3) * 256 + (((2 * (t & 7) + k_swap) ^ ((t >> 3) & 15)) << 4), vw_ch = (t & 3) * 32 + ((t >> 2) & 15);
+    const unsigned vw_off = 2 * KV4_KB + vw_ch * 128 + (((t >> 6) ^ ((vw_ch >> 1) & 7) ^ (vw_ch & 1) ^ ((t & 3) << 1)) << 4);
+    auto put_k = [&](auto W, const Kv4Stage<U>& x, int st) {               // word W of the units
+      constexpr int w = decltype(W)::value;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const unsigned byte = x.s[e >> 2] >> (8 * (e & 3)) & 255u;
-          const bool nan = byte >= 253u;
-          if (k0 + e >= nk || nan) x.s[e >> 2] &= ~(255u << (8 * (e & 3)));
-          if (k0 + e < nk && nan && vi == 0) atomicOr(&bad[st % 3][vt], 1ull << (vblk * 32 + vg * 8 + e));
-        }
-      }
-      const unsigned sc = x.ks << 23;
-      *reinterpret_cast<u32x4*>(kb + key * 256 + (((2 * part) ^ (key & 15)) << 4)) = fp4_word(x.k[0], sc);
-      *reinterpret_cast<u32x4*>(kb + key * 256 + (((2 * part + 1) ^ (key & 15)) << 4)) = fp4_word(x.k[1], sc);
-      u32x4 lo, hi;
-      fp4_octet(x.v, x.s, lo, hi);
-      const int ch = vt * 32 + vi, chunk = vblk * 4 + vg;
-      *reinterpret_cast<u32x4*>(vb + ch * 128 + ((chunk ^ ((ch >> 1) & 7)) << 4)) = lo;
-      *reinterpret_cast<u32x4*>(vb + (ch + 16) * 128 + ((chunk ^ (((ch + 16) >> 1) & 7)) << 4)) = hi;
+      for (int u = 0; u < U; ++u)                                           // unit t + 256: 32 keys on
+        *reinterpret_cast<u32x4*>(lds + ((kw_off + (st & 1) * KV4_KB) ^ (w << 4)) + u * 8192) = fp4_word(k_swap ? x.k[u][1 - w] : x.k[u][w], x.ks[u] << 23);
     };
-    if (t < 12) bad[t >> 2][t & 3] = 0ull;
+    auto put_v = [&](int u, const unsigned (&cv)[8], int st) {             // a unit's converted bytes; unit t + 256: four octets on
+      unsigned char* at = lds + ((vw_off + (st & 1) * KV4_VB) ^ (u << 6));
+      u32x4 v;
+#pragma unroll
+      for (int d = 0; d < 4; ++d) v[d] = __builtin_amdgcn_perm(cv[2 * d + 1], cv[2 * d], 0x05040100u);
+      *reinterpret_cast<u32x4*>(at) = v;
+#pragma unroll
+      for (int d = 0; d < 4; ++d) v[d] = __builtin_amdgcn_perm(cv[2 * d + 1], cv[2 * d], 0x07060302u);
+      *reinterpret_cast<u32x4*>(at + 2048) = v;
+    };
+    // What a row does not see must not reach it through 0 * NaN: values behind the last key become zeros, and NaN values zeros that are put into the rows that
+    // see them behind the product
+    auto hide = [&](Kv4Stage<U>& x, int st) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int key = ((t >> 6) + u * NW) * 8, left = nk - st * KV4_STAGE - key;         // of the stage: block, octet; keys of the octet that exist
+        const unsigned long long keep = left >= 8 ? ~0ull : left <= 0 ? 0ull : (1ull << (8 * left)) - 1;
+#pragma unroll
+        for (int d = 0; d < 2; ++d) {
+          const unsigned w = x.s[u][d] & (unsigned)(keep >> (32 * d));
+          const unsigned nan = ((w & 0x7f7f7f7fu) + 0x03030303u) & w & 0x80808080u;        // bytes of 253 and more
+          x.s[u][d] = w & ~((nan >> 7) * 255u);
+          if (nan && ((t >> 2) & 15) == 0)
+            atomicOr(&bad[st & 3][t & 3], (unsigned long long)((nan >> 7 & 1u) | (nan >> 14 & 2u) | (nan >> 21 & 4u) | (nan >> 28 & 8u)) << (key + 4 * d));
+        }
+      }
+    };
+    f32x16 sc[2];
+    bf16x8 pf[4];
+    float back = 1.f;
+    // operand of product i of a turn: V^T of stage st - 1 (i < 16: 16 keys i / 4, channels 32 (i mod 4) ..), K of stage st + 1 (key tile (i - 16) / 8, channels 16 (i mod 8) ..)
+    const unsigned v_off = 2 * KV4_KB + col * 128 + ((hh ^ ((col >> 1) & 7) ^ (col & 1)) << 4), k_row = swap23(col), k_off = k_row * 256 + ((hh ^ (k_row & 15)) << 4);
+    auto operand = [&](auto I, int st) -> u32x4 {
+      constexpr int i = decltype(I)::value;
+      if constexpr (i < 16) return *reinterpret_cast<const u32x4*>(lds + ((v_off + ((st + 1) & 1) * KV4_VB) ^ (((i >> 2) ^ (i & 3)) << 5)) + (i & 3) * 4096);
+      else return *reinterpret_cast<const u32x4*>(lds + ((k_off + ((st + 1) & 1) * KV4_KB) ^ ((i & 7) << 5)) + ((i - 16) >> 3) * 8192);
+    };
+    auto product = [&](auto I, const u32x4& x) {
+      constexpr int i = decltype(I)::value;
+      if constexpr (i < 16) o[i & 3] = mfma32(as_bf16x8(x), pf[i >> 2], o[i & 3]);
+      else {
+        constexpr int T = (i - 16) >> 3;
+        if constexpr ((i & 7) == 0) {
+#pragma unroll
+          for (int z = 0; z < 16; ++z) sc[T][z] = 0.f;
+        }
+        sc[T] = mfma32(as_bf16x8(x), as_bf16x8(qf[i & 7]), sc[T]);
+      }
+    };
+    // NaN values of a stage into the rows that see them
+    auto put_nan = [&](int st) {
+      const int seen = lim - st * KV4_STAGE;                                // keys 0 .. seen of the stage
+      const unsigned long long mine = seen >= 63 ? ~0ull : seen < 0 ? 0ull : (2ull << seen) - 1;
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        const bool put = (bad[st & 3][d] & mine) != 0;
+        if (__any(put)) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[d][i] = put ? __builtin_nanf("") : o[d][i];
+        }
+      }
+    };
+
+    Kv4Stage<U> x;
+    const int top_st = s1 - 1;
+    if (t < 16) bad[t >> 2][t & 3] = 0ull;
+    const std::integral_constant<int, 0> first; const std::integral_constant<int, 1> second;
+    {                                                                       // all in flight at once
+      Kv4Stage<U> y, z;
+      fetch_k(y, s0);
+      fetch_k(z, min(s0 + 1, top_st));
+      fetch_k(x, min(s0 + 2, top_st));
+      fetch_v(x, s0);
+      put_k(first, y, s0); put_k(second, y, s0);
+      put_k(first, z, s0 + 1); put_k(second, z, s0 + 1);
+    }
+    for (int i = t; i < KV4_VB / 16; i += NW * 64)                          // the stage before the first
+      *reinterpret_cast<u32x4*>(lds + 2 * KV4_KB + ((s0 + 1) & 1) * KV4_VB + i * 16) = (u32x4){0, 0, 0, 0};
+#pragma unroll
+    for (int u = 0; u < 4; ++u) pf[u] = as_bf16x8((u32x4){0, 0, 0, 0});
     __syncthreads();
-    Kv4Stage x;
-    fetch(x, s0);
-    stage(x, s0);
-    if (s0 + 1 < s1) fetch(x, s0 + 1);
-    __syncthreads();
-    const int krow = swap23(col);
+    unrolled<16>([&](auto I) { const std::integral_constant<int, 16 + decltype(I)::value> J; product(J, operand(J, s0 - 1)); });
+    __syncthreads();                                                        // K of the first stage is read before its slot is filled again
+    // A turn: the softmax of stage st beside the products that do not wait for it, P V of the stage before and K Q^T of the one behind; K of st + 2 and V of
+    // st go to LDS, those of the turn behind are fetched.
     for (int st = s0; st < s1; ++st) {
-      const unsigned char* kb = lds + (st & 1) * (KV4_KB + KV4_VB);
-      const unsigned char* vb = kb + KV4_KB;
-      if (t < 4) bad[(st + 2) % 3][t] = 0ull;                               // last read one stage ago, next written one stage on
-      f32x16 sc[2];
-      if (active) {
+      if (masked(st)) {
 #pragma unroll
-        for (int T = 0; T < 2; ++T) {
+        for (int T = 0; T < 2; ++T)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) sc[T][i] = 0.f;
-          const int row = T * 32 + krow;
-#pragma unroll
-          for (int s = 0; s < 8; ++s)
-            sc[T] = mfma32(as_bf16x8(*reinterpret_cast<const u32x4*>(kb + row * 256 + (((2 * s + hh) ^ (row & 15)) << 4))), as_bf16x8(qf[s]), sc[T]);
-        }
+          for (int i = 0; i < 16; ++i) sc[T][i] = st * KV4_STAGE + T * 32 + (i >> 3) * 16 + hh * 8 + (i & 7) <= lim ? sc[T][i] : -INFINITY;
+        hide(x, st);
+        if (st - 2 >= s0 && masked(st - 2)) put_nan(st - 2);                // O holds the stages up to that one
       }
-      if (st + 1 < s1) { stage(x, st + 1); if (st + 2 < s1) fetch(x, st + 2); }
-      if (active) {
-        if (masked(st)) {
+      if (__any(back != 1.f)) {                                             // the maximum has moved in the turn before: O is one stage behind
 #pragma unroll
-          for (int T = 0; T < 2; ++T)
+        for (int d = 0; d < 4; ++d) o[d] *= back;
+      }
+      if (t < 4) bad[(st + 1) & 3][t] = 0ull;                               // last read a turn ago, next written a turn on
+      // 32 products, their operands read four ahead, and the vector work dealt out between them
+      u32x4 fr[5], pn[4];
+      unsigned cv[8];
+      float t0 = 0.f, t1 = 0.f, mu = 0.f, f = 1.f;
+      unrolled<4>([&](auto I) { fr[decltype(I)::value] = operand(I, st); });
+      unrolled<32>([&](auto I) {
+        constexpr int i = decltype(I)::value;
+        if constexpr (i + 4 < 32) fr[(i + 4) % 5] = operand(std::integral_constant<int, i + 4>{}, st);
+        product(I, fr[i % 5]);
+        if constexpr (i < 2) {
+          float& tt = i == 0 ? t0 : t1;
+          tt = sc[i][0];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) sc[T][i] = st * KV4_STAGE + T * 32 + (i >> 3) * 16 + hh * 8 + (i & 7) <= lim ? sc[T][i] : -INFINITY;
-        }
-        float top = sc[0][0];
-#pragma unroll
-        for (int i = 1; i < 32; ++i) top = __builtin_fmaxf(top, sc[i >> 4][i & 15]);
-        top = xor32_max(top);
-        const float mn = __builtin_fmaxf(m, top * scale_log2e), mu = mn == -INFINITY ? 0.f : mn;
-        if (__any(mn > m)) {
-          const float f = __builtin_amdgcn_exp2f(m - mu);
-          l *= f;
-#pragma unroll
-          for (int d = 0; d < 4; ++d) o[d] *= f;
+          for (int z = 1; z < 16; ++z) tt = __builtin_fmaxf(tt, sc[i][z]);
+        } else if constexpr (i == 2) {
+          const float top = xor32_max(__builtin_fmaxf(t0, t1)) * scale_log2e;
+          const float mn = top > m + KV4_SLACK ? top : m;
+          mu = mn == -INFINITY ? 0.f : mn;
+          f = __builtin_amdgcn_exp2f(m - mu);
           m = mn;
-        }
+          l *= f;
+        } else if constexpr (i < 19) {                                      // two probabilities: the first tile's before its scores are overwritten, the second's too
+          constexpr int k = i - 3;
+          const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[k >> 3][(2 * k) & 15], scale_log2e, -mu)), p1 = __builtin_amdgcn_exp2f(fmaf(sc[k >> 3][(2 * k + 1) & 15], scale_log2e, -mu));
+          l += p0 + p1;
+          pn[k >> 2][k & 3] = pack2(p0, p1);
+        } else if constexpr (i < 19 + 2 * U) {                              // V a unit at a time: converted, put
+          constexpr int u = (i - 19) >> 1;
+          if constexpr (((i - 19) & 1) == 0) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          float p[8];
+            for (int d = 0; d < 2; ++d) {
+              cv[4 * d] = fp4_pair<0>(x.v[u][d], scale_of<0>(x.s[u][d])); cv[4 * d + 1] = fp4_pair<1>(x.v[u][d], scale_of<1>(x.s[u][d]));
+              cv[4 * d + 2] = fp4_pair<2>(x.v[u][d], scale_of<2>(x.s[u][d])); cv[4 * d + 3] = fp4_pair<3>(x.v[u][d], scale_of<3>(x.s[u][d]));
+            }
+          } else put_v(u, cv, st);
+        } else if constexpr (i >= 23 && i < 25) put_k(std::integral_constant<int, i - 23>{}, x, st + 2);
+        else if constexpr (i == 25) fetch_k(x, min(st + 3, top_st));
+        else if constexpr (i == 27) fetch_v(x, min(st + 1, top_st));
+      });
 #pragma unroll
-          for (int e = 0; e < 8; ++e) { p[e] = __builtin_amdgcn_exp2f(fmaf(sc[u >> 1][(u & 1) * 8 + e], scale_log2e, -mu)); l += p[e]; }
-          const bf16x8 pf = as_bf16x8((u32x4){pack2(p[0], p[1]), pack2(p[2], p[3]), pack2(p[4], p[5]), pack2(p[6], p[7])});
-#pragma unroll
-          for (int d = 0; d < 4; ++d) {
-            const int row = d * 32 + col;
-            o[d] = mfma32(as_bf16x8(*reinterpret_cast<const u32x4*>(vb + row * 128 + (((2 * u + hh) ^ ((row >> 1) & 7)) << 4))), pf, o[d]);
-          }
-        }
-        if (masked(st)) {
-          const int seen = lim - st * KV4_STAGE;                            // keys 0 .. seen of the stage
-          const unsigned long long mine = seen >= 63 ? ~0ull : seen < 0 ? 0ull : (2ull << seen) - 1;
-#pragma unroll
-          for (int d = 0; d < 4; ++d)
-            if (bad[st % 3][d] & mine)
-#pragma unroll
-              for (int i = 0; i < 16; ++i) o[d][i] = __builtin_nanf("");
-        }
-      }
+      for (int u = 0; u < 4; ++u) pf[u] = as_bf16x8(pn[u]);
+      back = f;
       __syncthreads();
     }
+    if (top_st - 1 >= s0 && masked(top_st - 1)) put_nan(top_st - 1);
+#pragma unroll
+    for (int d = 0; d < 4; ++d) o[d] *= back;
+    unrolled<16>([&](auto I) { product(I, operand(I, top_st + 1)); });
+    if (masked(top_st)) put_nan(top_st);
     l = xor32_sum(l);
   }
   if (!valid) return;
@@ -604,20 +734,32 @@ __global__ __launch_bounds__(512, 2) void attn_prefill_kv4_kernel(Kv4Args a, con
   }
 }
 
+// Tile height and key splits.  Blocks of eight waves (256 columns), one a compute unit; where no stream has more than 128 columns, of four waves, two a unit.  Cost in
+// stages of 64 keys (1.6 us in either): a block's prologue and result count as 2.5; blocks that all run at once take as long as the longest, more of them the mean
+// plus most of one; the join costs a launch (2 stages) and its partials written and read (1,040 bytes a row, head and split at 4.5 TB/s).
 int kv4_prefill_plan(const int32_t* n_new, const int32_t* past, int n, int n_q_heads, int n_kv_heads, int cus, int* tile_rows, int* nsplit) {
   if (n < 0 || n_q_heads < 1 || n_kv_heads < 1 || n_q_heads % n_kv_heads || n_q_heads / n_kv_heads > 16 || cus < 1) return LCC_ERR_SHAPE;
-  const int rows = 256 / (n_q_heads / n_kv_heads);
-  long tiles = 0, keys = 0;
+  const int G = n_q_heads / n_kv_heads;
+  long most = 0, rows = 0;
   for (int i = 0; i < n; ++i) {
     if (n_new[i] < 0 || past[i] < 0) return LCC_ERR_SHAPE;
-    tiles += (n_new[i] + rows - 1) / rows;
-    if (n_new[i] > 0 && (long)past[i] + n_new[i] > keys) keys = (long)past[i] + n_new[i];
+    most = std::max(most, (long)n_new[i]);
+    rows += n_new[i];
   }
-  const long base = tiles * n_kv_heads, stages = (keys + KV4_STAGE - 1) / KV4_STAGE;
-  *tile_rows = rows; *nsplit = 1;
+  const bool small = most * G <= 128;
+  const int height = (small ? 128 : 256) / G;
+  long tiles = 0, total = 0, longest = 0;
+  for (int i = 0; i < n; ++i)
+    for (long r = 0; r < n_new[i]; r += height) {
+      const long st = (past[i] + std::min<long>(n_new[i], r + height) + KV4_STAGE - 1) / KV4_STAGE;
+      ++tiles; total += st; longest = std::max(longest, st);
+    }
+  const float slots = (float)cus * (small ? 2 : 1), join = rows * (float)n_q_heads * (1040.f / 4.5e6f / 1.6f);
+  *tile_rows = height; *nsplit = 1;
   float best = 1e30f;
-  for (int k = 1; k <= 32 && k <= (stages + 3) / 4; ++k) {
-    const float cost = (float)((base * k + cus - 1) / cus) * ((float)stages / k + 3.f) + (k > 1 ? 4.f + 0.5f * k : 0.f);
+  for (int k = 1; k <= 64 && k <= std::max(1L, longest / 4); ++k) {
+    const float block = (float)longest / k + 2.5f, blocks = (float)tiles * n_kv_heads * k;
+    const float cost = (blocks <= slots ? block : (total * (float)n_kv_heads + 2.5f * blocks) / slots + 0.8f * block) + (k > 1 ? 2.f + join * k : 0.f);
     if (cost < best) { best = cost; *nsplit = k; }
   }
   return 0;
@@ -626,16 +768,23 @@ int kv4_prefill_plan(const int32_t* n_new, const int32_t* past, int n, int n_q_h
 int attn_prefill_kv4(const Kv4Args& a, const bf16_t* q, bf16_t* out, const int32_t* tile_stream, const int32_t* tile_q0, const int32_t* tile_nq, const int32_t* tile_pos0,
                      int n_tiles, int n_q_heads, int tile_rows, int nsplit, int n_rows, float* ws_o, float* ws_ml, hipStream_t st) {
   if (int rc = a.check()) return rc;
-  if (n_tiles < 0 || n_tiles > 65535 || n_rows < 0 || n_q_heads < 1 || n_q_heads % a.n_kv_heads || n_q_heads / a.n_kv_heads > 16 || nsplit < 1 || nsplit > 32)
+  if (n_tiles < 0 || n_tiles > 65535 || n_rows < 0 || n_q_heads < 1 || n_q_heads % a.n_kv_heads || n_q_heads / a.n_kv_heads > 16 || nsplit < 1 || nsplit > 64)
     return LCC_ERR_SHAPE;
   if (tile_rows < 1 || tile_rows > 256 / (n_q_heads / a.n_kv_heads)) return LCC_ERR_SHAPE;
   if (nsplit > 1 && (ws_o == nullptr || ws_ml == nullptr)) return LCC_ERR_ARG;
   if (n_tiles == 0 || n_rows == 0) return 0;
   static DeviceOnce once;
-  if (once.first()) (void)hipFuncSetAttribute((const void*)attn_prefill_kv4_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, KV4_LDS);
-  attn_prefill_kv4_kernel<<<dim3(a.n_kv_heads, n_tiles, nsplit), dim3(512), KV4_LDS, st>>>(a, q, out, tile_stream, tile_q0, tile_nq, tile_pos0, n_q_heads, tile_rows,
-                                                                                          nsplit, n_rows, ws_o, ws_ml, 1.4426950408889634f / sqrtf(128.f));
-  if (nsplit > 1) kv4_combine_kernel<<<dim3((unsigned)n_rows * n_q_heads), dim3(256), 0, st>>>(ws_o, ws_ml, out, nsplit);
+  if (once.first()) {
+    (void)hipFuncSetAttribute((const void*)attn_prefill_kv4_kernel<8>, hipFuncAttributeMaxDynamicSharedMemorySize, KV4_LDS);
+    (void)hipFuncSetAttribute((const void*)attn_prefill_kv4_kernel<4>, hipFuncAttributeMaxDynamicSharedMemorySize, KV4_LDS);
+  }
+  const dim3 grid(a.n_kv_heads, n_tiles, nsplit);
+  const float scale = 1.4426950408889634f / sqrtf(128.f);
+  if (tile_rows * (n_q_heads / a.n_kv_heads) > 128)
+    attn_prefill_kv4_kernel<8><<<grid, dim3(512), KV4_LDS, st>>>(a, q, out, tile_stream, tile_q0, tile_nq, tile_pos0, n_q_heads, tile_rows, nsplit, n_rows, ws_o, ws_ml, scale);
+  else
+    attn_prefill_kv4_kernel<4><<<grid, dim3(256), KV4_LDS, st>>>(a, q, out, tile_stream, tile_q0, tile_nq, tile_pos0, n_q_heads, tile_rows, nsplit, n_rows, ws_o, ws_ml, scale);
+  if (nsplit > 1) kv4_combine(ws_o, ws_ml, out, (int64_t)n_rows * n_q_heads, nsplit, st);
   return 0;
 }
 

@@ -260,6 +260,7 @@ Tensor qk_norm_rope_kv_append(const optional<Tensor>& qkv, const optional<Tensor
   const bool have_qkv = qkv.has_value() && qkv->defined(), have_part = partial.has_value() && partial->defined();
   TORCH_CHECK(have_qkv != have_part, "qk_norm_rope_kv_append: exactly one of qkv (bf16 [S, (Hq+2Hkv)*128]) and partial (fp32 [NS, S, ...]) is needed");
   TORCH_CHECK(n_q_heads >= 0 && n_q_heads <= 65535 && S <= 0x7fffffff, "qk_norm_rope_kv_append: bad n_q_heads / rows");
+  TORCH_CHECK(eps > 0 || !((q_norm.has_value() && q_norm->defined()) || (k_norm.has_value() && k_norm->defined())), "qk_norm_rope_kv_append: eps must be positive");
   const int64_t width = (n_q_heads + 2 * n_kv_heads) * 128;
   if (have_qkv) { TORCH_CHECK(qkv->dim() == 2 && qkv->size(0) == S && qkv->size(1) == width, "qk_norm_rope_kv_append: qkv must be [S, (Hq+2Hkv)*128]"); same_device(cos, *qkv, "qkv"); }
   if (have_part) {
@@ -321,7 +322,7 @@ Tensor attn_prefill4(const Tensor& q, const Tensor& kv_ptrs, const Tensor& kv_bu
   TORCH_CHECK(n_q_heads >= 1 && n_q_heads % n_kv_heads == 0 && n_q_heads / n_kv_heads <= 16, "attn_prefill4: up to 16 query heads per KV head");
   TORCH_CHECK(q.dim() == 2 && q.size(1) == n_q_heads * 128 && q.size(0) <= 0x7fffffff / n_q_heads, "attn_prefill4: q must be [S, Hq*128]");
   TORCH_CHECK(tiles.dim() == 2 && tiles.size(0) == 4 && tiles.size(1) <= 65535, "attn_prefill4: tiles must be int32 [4, n <= 65535]: slot, first row, rows, first position");
-  TORCH_CHECK(tile_rows >= 1 && tile_rows <= 256 / (n_q_heads / n_kv_heads) && nsplit >= 1 && nsplit <= 32, "attn_prefill4: bad tile_rows / nsplit");
+  TORCH_CHECK(tile_rows >= 1 && tile_rows <= 256 / (n_q_heads / n_kv_heads) && nsplit >= 1 && nsplit <= 64, "attn_prefill4: bad tile_rows / nsplit");
   const int64_t S = q.size(0), nt = tiles.size(1);
   const int32_t* t = index_ptr(q, tiles, 4 * nt, false, "tiles");
   Tensor out = at::empty_like(q), ws;

@@ -469,15 +469,12 @@ def qk_norm_rope_kv_append(qkv: Optional[torch.Tensor], cos, sin, tok_stream, to
     """`rope_kv_append` with RMS norms of the query and key heads (weights [128], None: no norm) in front of the rotation, into a `KvArena` or a `Kv4Arena`;
     returns the queries [S, Hq*128].  A row whose `tok_stream` is out of range (-1: padding) or whose position is behind the arena appends nothing.  (slot,
     position) pairs of a call must be distinct."""
+    if cos.is_cuda:
+        t = _T.op("qk_norm_rope_kv_append")                 # checks its arguments itself
+        if t is not None:
+            return t(qkv, partial, bias, q_norm, k_norm, eps, cos, sin, tok_stream, tok_pos, kv_len, kv.ptrs, kv.buf, kv.n_layers, kv.n_kv_heads, kv.lmax, layer, n_q_heads)
     for a, dt, nm in ((qkv, torch.bfloat16, "qkv"), (partial, torch.float32, "partial"), (cos, torch.bfloat16, "cos"), (tok_stream, torch.int32, "tok_stream")):
         _chk(a, dt, nm)
-    if cos.shape[0] == 0 or (q_norm is None and k_norm is None) or eps > 0:
-        t = _T.op("qk_norm_rope_kv_append")
-        if t is not None:
-            return t(qkv, partial, bias, q_norm, k_norm, float(eps), cos, sin, tok_stream, tok_pos, kv_len, kv.ptrs, kv.buf, kv.n_layers, kv.n_kv_heads, kv.lmax,
-                     int(layer), int(n_q_heads))
-    else:
-        raise ValueError("qk_norm_rope_kv_append: eps must be positive")
     S, width = cos.shape[0], (n_q_heads + 2 * kv.n_kv_heads) * 128
     n_slots = kv.buf.shape[0]
     _same_device(cos, sin=sin, tok_stream=tok_stream, tok_pos=tok_pos, kv_len=kv_len, qkv=qkv, partial=partial, bias=bias, q_norm=q_norm, k_norm=k_norm, kv=kv.buf)
@@ -522,10 +519,11 @@ def _kv4(kv) -> None:
 def kv4_read(kv: Kv4Arena, layer: int, tok_stream: torch.Tensor, tok_pos: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """Keys and values [S, Hkv, 128] (bf16) of S (slot, position) pairs out of the 4-bit cache; zeros where a pair is out of range."""
     _kv4(kv)
+    if tok_stream.is_cuda:
+        t = _T.op("kv4_read")
+        if t is not None:
+            return t(kv.ptrs, kv.buf, kv.n_layers, kv.n_kv_heads, kv.lmax, layer, tok_stream, tok_pos)
     _chk(tok_stream, torch.int32, "tok_stream"), _chk(tok_pos, torch.int32, "tok_pos")
-    t = _T.op("kv4_read")
-    if t is not None:
-        return t(kv.ptrs, kv.buf, kv.n_layers, kv.n_kv_heads, kv.lmax, int(layer), tok_stream, tok_pos)
     S = tok_stream.numel()
     _same_device(tok_stream, tok_pos=tok_pos, kv=kv.buf), _shape(tok_stream, (S,), "tok_stream"), _shape(tok_pos, (S,), "tok_pos")
     k = torch.empty(S, kv.n_kv_heads, 128, dtype=torch.bfloat16, device=kv.buf.device)
@@ -550,12 +548,13 @@ def attn_decode4(q: torch.Tensor, kv: Kv4Arena, layer: int, slots: torch.Tensor,
     """`attn_decode` over the 4-bit cache: row b sees keys 0 .. kv_len[slots[b]] of its slot (none at -1, or for a slot out of range: zeros).  nsplit 0: the split
     count that suits streams as long as the arena; callers that know the lengths take it from `kv4_decode_splits`."""
     _kv4(kv)
-    _chk(q, torch.bfloat16, "q"), _chk(slots, torch.int32, "slots"), _chk(kv_len, torch.int32, "kv_len")
     if nsplit == 0:
         nsplit = kv4_decode_splits([kv.lmax] * max(1, q.shape[0]), kv.n_kv_heads)
-    t = _T.op("attn_decode4")
-    if t is not None:
-        return t(q, kv.ptrs, kv.buf, kv.n_layers, kv.n_kv_heads, kv.lmax, int(layer), slots, kv_len, int(n_q_heads), int(nsplit))
+    if q.is_cuda:
+        t = _T.op("attn_decode4")
+        if t is not None:
+            return t(q, kv.ptrs, kv.buf, kv.n_layers, kv.n_kv_heads, kv.lmax, layer, slots, kv_len, n_q_heads, nsplit)
+    _chk(q, torch.bfloat16, "q"), _chk(slots, torch.int32, "slots"), _chk(kv_len, torch.int32, "kv_len")
     B, n_slots = q.shape[0], kv.buf.shape[0]
     _same_device(q, slots=slots, kv_len=kv_len, kv=kv.buf), _shape(q, (B, n_q_heads * 128), "q"), _shape(slots, (B,), "slots")
     if kv_len.numel() < n_slots:
@@ -602,14 +601,15 @@ def attn_prefill4(q: torch.Tensor, kv: Kv4Arena, layer: int, plan, n_q_heads: in
     _kv4(kv)
     if not isinstance(plan, Kv4PrefillPlan):
         plan = Kv4PrefillPlan(plan, n_q_heads, kv.n_kv_heads, q.device)
-    _chk(q, torch.bfloat16, "q"), _chk(plan.tiles, torch.int32, "plan")
     if plan.rows != q.shape[0] or plan.n_q_heads != n_q_heads or plan.n_kv_heads != kv.n_kv_heads:
         raise ValueError(f"attn_prefill4: the plan is of {plan.rows} rows, {plan.n_q_heads} / {plan.n_kv_heads} heads")
     if plan.max_keys > kv.lmax:
         raise ValueError(f"attn_prefill4: {plan.max_keys} keys, the arena holds {kv.lmax}")
-    t = _T.op("attn_prefill4")
-    if t is not None:
-        return t(q, kv.ptrs, kv.buf, kv.n_layers, kv.n_kv_heads, kv.lmax, int(layer), plan.tiles, int(n_q_heads), plan.tile_rows, plan.nsplit)
+    if q.is_cuda:
+        t = _T.op("attn_prefill4")
+        if t is not None:
+            return t(q, kv.ptrs, kv.buf, kv.n_layers, kv.n_kv_heads, kv.lmax, layer, plan.tiles, n_q_heads, plan.tile_rows, plan.nsplit)
+    _chk(q, torch.bfloat16, "q"), _chk(plan.tiles, torch.int32, "plan")
     S, nt = q.shape[0], plan.tiles.shape[1]
     _same_device(q, plan=plan.tiles, kv=kv.buf), _shape(q, (S, n_q_heads * 128), "q")
     out = torch.empty_like(q)

@@ -493,7 +493,7 @@ def test_refusals(dev, through, monkeypatch):
                 lambda: ops.attn_decode4(rand((S, 34 * 128), dev, 1), kv, 0, st, pos, 34),
                 lambda: ops.attn_prefill4(qkv[:, :512].contiguous(), kv, 0, [(0, 2, 0)], heads),
                 lambda: ops.attn_prefill4(qkv[:, :512].contiguous(), kv, 0, [(0, 3, 62)], heads),
-                lambda: ops.attn_prefill4(qkv[:, :512].contiguous(), kv, 0, ops.kv4_prefill_plan([(0, 3, 0)], heads, kv_heads, dev, 33), heads),
+                lambda: ops.attn_prefill4(qkv[:, :512].contiguous(), kv, 0, ops.kv4_prefill_plan([(0, 3, 0)], heads, kv_heads, dev, 65), heads),
                 lambda: ops.attn_prefill4(qkv[:, :512].contiguous(), kv, 0, ops.kv4_prefill_plan([(0, 3, 0)], 8, kv_heads, dev), heads)):
         with pytest.raises(err):
             bad()

@@ -89,7 +89,7 @@ def test_prefill_plans(built_lib, heads, kv_heads):
     from livecc_amd import ops
     seg = [(2, 386, 6120), (0, 0, 5), (1, 1, 0), (4, 37, 12)]
     plan = ops.kv4_prefill_plan(seg, heads, kv_heads, "cpu")
-    assert plan.rows == 424 and plan.max_keys == 6506 and 1 <= plan.nsplit <= 32 and 1 <= plan.tile_rows <= 256 // (heads // kv_heads)
+    assert plan.rows == 424 and plan.max_keys == 6506 and 1 <= plan.nsplit <= 64 and 1 <= plan.tile_rows <= 256 // (heads // kv_heads)
     rows = [None] * plan.rows
     for slot, q0, nq, pos0 in plan.tiles.T.tolist():
         assert 1 <= nq <= plan.tile_rows
@@ -153,7 +153,7 @@ def test_c_entries_refuse_before_any_launch(built_lib):
         return lib.lcc_attn_prefill_kv4(*a.values(), None)
     assert [chunk(**{n: None}) for n in ("q", "out", "t0", "t1", "t2", "t3", "base")] == [ERR_ARG] * 7
     assert chunk(nsplit=2) == ERR_ARG
-    for kw in (dict(H=3), dict(H=34), dict(nsplit=0), dict(nsplit=33, o=p, ml=p), dict(tiles=-1), dict(tiles=65536), dict(rows=0), dict(rows=129), dict(S=-1), dict(layer=1)):
+    for kw in (dict(H=3), dict(H=34), dict(nsplit=0), dict(nsplit=65, o=p, ml=p), dict(tiles=-1), dict(tiles=65536), dict(rows=0), dict(rows=129), dict(S=-1), dict(layer=1)):
         assert chunk(**kw) == ERR_SHAPE, kw
     assert chunk(q=odd) == chunk(out=odd) == ERR_ALIGN
 
