@@ -131,6 +131,7 @@ LCC_DEVICE void row8(const QkNormArgs& a, int s, int col, float* v) {
 // RMS norm of a head's 128 channels over its eight lanes, with the model's rounding points: bf16(w bf16(x r)).  The mean square and its root are formed in 64
 // bits and r is rounded once: keys are quantised behind this, and codes must not depend on the order of a sum.
 LCC_DEVICE void head_norm(float (&x1)[8], float (&x2)[8], const bf16_t* w, int c0, float eps) {
+  const u32x4 w1 = ld16(w + c0), w2 = ld16(w + c0 + 64);
   double ss = 0.0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) { ss = fma((double)x1[e], (double)x1[e], ss); ss = fma((double)x2[e], (double)x2[e], ss); }
@@ -140,93 +141,223 @@ LCC_DEVICE void head_norm(float (&x1)[8], float (&x2)[8], const bf16_t* w, int c
   double r = __builtin_amdgcn_rsq(m);
   if (m < __builtin_inf()) r = fma(0.5 * r, fma(-m * r, r, 1.0), r);        // the unit's result is good to about 2^-28; one step squares that
   const float rf = (float)r;
-  const u32x4 w1 = ld16(w + c0), w2 = ld16(w + c0 + 64);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float a = (e & 1) ? hi2f(w1[e >> 1]) : lo2f(w1[e >> 1]), b = (e & 1) ? hi2f(w2[e >> 1]) : lo2f(w2[e >> 1]);
-    x1[e] = rbf(a * rbf(x1[e] * rf));
-    x2[e] = rbf(b * rbf(x2[e] * rf));
+  for (int d = 0; d < 4; ++d) {
+    float *a = x1 + 2 * d, *b = x2 + 2 * d;
+    a[0] *= rf; a[1] *= rf; b[0] *= rf; b[1] *= rf;
+    rbf2(a[0], a[1]); rbf2(b[0], b[1]);
+    a[0] *= lo2f(w1[d]); a[1] *= hi2f(w1[d]); b[0] *= lo2f(w2[d]); b[1] *= hi2f(w2[d]);
+    rbf2(a[0], a[1]); rbf2(b[0], b[1]);
   }
 }
 
-// Eight lanes a (row, head): lane j holds channels 8 j .. + 7 and 64 + 8 j .. + 7, the rotation's pairs and, four lanes each, two groups of the 4-bit
-// format (2 shuffles a group, 3 for the norm).
-template <bool KV4>
-__global__ __launch_bounds__(256) void qk_norm_rope_append_kernel(QkNormArgs a) {
-  const int per_row = a.n_q_heads + 2 * a.n_kv_heads;
-  const int64_t item = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3);
-  if (item >= (int64_t)a.rows * per_row) return;                            // whole groups of eight lanes
-  const int s = (int)(item / per_row), head = (int)(item - (int64_t)s * per_row), j = threadIdx.x & 7, c0 = j * 8;
-  const int kind = head < a.n_q_heads ? 0 : head < a.n_q_heads + a.n_kv_heads ? 1 : 2, h = kind == 0 ? head : (head - a.n_q_heads) - (kind - 1) * a.n_kv_heads;
+// From so many rows on V goes by windows: 1,131 rows of 28 / 4 heads 11.5 -> 9.0 us (4 bits 9.3 -> 8.3), 9,048 rows 62 -> 48 (46.6 -> 42.8); 386 rows 5.9 either way, 100 rows 4.4
+// against 5.1
+constexpr int KV4_WINDOW_ROWS = 512;
+// Where a row's keys and values go: its slot and position, slot -1 for a row of no stream or no position.
+LCC_DEVICE void row_place(const QkNormArgs& a, int s, int& slot, int& pos) {
+  slot = a.tok_stream[s];
+  pos = -1;
+  if (slot >= 0 && slot < a.n_slots) pos = a.tok_pos != nullptr ? a.tok_pos[s] : a.kv_len[slot];
+  if (pos < 0 || pos >= a.lmax) slot = -1;
+}
+// The lane's V codes: channels i and 16 + i of a group lie two lanes apart, so of four lanes the lower pair takes the lower group's bytes (r1: group j / 4), the
+// upper pair the upper group's (2 + j / 4): bytes i = 8 (j & 1) .. + 7 of group t, e its scale
+LCC_DEVICE void v_codes(const u32x4& r1, const u32x4& r2, int j, u32x2& bytes, int& t, int& e) {
+  const int e1 = kv4_exponent(max4(max_bits(r1))), e2 = kv4_exponent(max4(max_bits(r2)));
+  const unsigned w1 = fp4_of(r1, e1), w2 = fp4_of(r2, e2);
+  const bool up = (j & 2) != 0;
+  const unsigned mine = up ? w2 : w1, other = __shfl_xor(up ? w1 : w2, 2, 64), lo = up ? other : mine, hi = up ? mine : other;
+  t = up ? 2 + (j >> 2) : j >> 2;
+  e = up ? e2 : e1;
+#pragma unroll
+  for (int d = 0; d < 2; ++d) {                       // nibbles 4 d .. 4 d + 3 of either word, spread to bytes
+    const unsigned a = lo >> (16 * d) & 0xffffu, b = hi >> (16 * d) & 0xffffu;
+    const unsigned x = (a | a << 8) & 0x00ff00ffu, y = (b | b << 8) & 0x00ff00ffu;
+    bytes[d] = ((x | x << 4) & 0x0f0f0f0fu) | ((y | y << 4) & 0x0f0f0f0fu) << 4;
+  }
+}
+// 16 channels of a row: a lane's r1, r2
+LCC_DEVICE void row_pairs(const QkNormArgs& a, int s, int col, u32x4& r1, u32x4& r2) {
   float x1[8], x2[8];
-  row8(a, s, head * 128 + c0, x1);
-  row8(a, s, head * 128 + 64 + c0, x2);
+  row8(a, s, col, x1);
+  row8(a, s, col + 64, x2);
+#pragma unroll
+  for (int d = 0; d < 4; ++d) { r1[d] = pack2(x1[2 * d], x1[2 * d + 1]); r2[d] = pack2(x2[2 * d], x2[2 * d + 1]); }
+}
+
+// V of 32 consecutive rows of a KV head, a block: V lies position-innermost, so rows are turned in LDS.  Where the rows are consecutive positions of one stream (a chunk
+// but for its ends) each run of eight aligned positions is one store of a channel (16 bytes of bf16; 4 bits: 8 of a channel pair), else positions are stored one by one.
+template <bool KV4>
+LCC_DEVICE void append_v_window(const QkNormArgs& a, int h, int r0, unsigned char* lds) {
+  constexpr int PITCH = KV4 ? 68 : 260;                                     // bytes of a row: 64 code bytes [t][i] and 4 scales, or 128 bf16 (+ 4: rows on other banks)
+  const int tid = threadIdx.x, row = tid >> 3, j = tid & 7, n = min(32, a.rows - r0), lane = tid & 63;
+  u32x4 r1, r2;
+  row_pairs(a, r0 + min(row, n - 1), (a.n_q_heads + a.n_kv_heads + h) * 128 + j * 8, r1, r2);
+  int slot, pos;
+  row_place(a, r0 + min(lane & 31, n - 1), slot, pos);
+  unsigned char* at = lds + row * PITCH;
+  if (KV4) {
+    u32x2 w; int t, e;
+    v_codes(r1, r2, j, w, t, e);
+    *reinterpret_cast<unsigned*>(at + t * 16 + (j & 1) * 8) = w[0];
+    *reinterpret_cast<unsigned*>(at + t * 16 + (j & 1) * 8 + 4) = w[1];
+    if ((j & 1) == 0) at[64 + t] = (unsigned char)e;
+  } else {
+#pragma unroll
+    for (int d = 0; d < 4; ++d) { *reinterpret_cast<unsigned*>(at + j * 16 + 4 * d) = r1[d]; *reinterpret_cast<unsigned*>(at + 128 + j * 16 + 4 * d) = r2[d]; }
+  }
+  const int slot0 = __builtin_amdgcn_readfirstlane(slot), pos0 = __builtin_amdgcn_readfirstlane(pos);
+  const bool chunk = __all((lane & 31) >= n || (slot0 >= 0 && slot == slot0 && pos == pos0 + (lane & 31)));
+  __syncthreads();
+  const Kv4Layout lay{a.n_kv_heads, a.lmax};
+  const size_t kv = (size_t)a.n_kv_heads * a.lmax * 128;
+  auto base_of = [&](int sl) -> uint8_t* {
+    return KV4 ? (uint8_t*)a.kv_base[sl] + (size_t)a.layer * lay.layer_bytes() : (uint8_t*)((bf16_t*)a.kv_base[sl] + ((size_t)a.layer * 2 + 1) * kv + (size_t)h * a.lmax * 128);
+  };
+  // a thread turns one word of eight rows: four bytes' units of eight positions (code bytes 4 (u mod 4) .. + 3 of group u / 4; u = 16: the scales), or a pair of channels
+  constexpr int UNITS = KV4 ? 17 : 64;
+  const int shift = chunk ? pos0 & 7 : 0, octets = (shift + n + 7) / 8;
+  for (int i = tid; i < octets * UNITS; i += 256) {
+    const int oct = i / UNITS, u = i - oct * UNITS;
+    const int first = oct * 8 - shift, e0 = max(0, -first), e1 = min(8, n - first);         // rows first + e0 .. first + e1 - 1 of the window
+    unsigned x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = *reinterpret_cast<const unsigned*>(lds + min(max(first + e, 0), 31) * PITCH + u * 4);
+    auto place4 = [&](uint8_t* base, int ps, int z) -> uint8_t* {           // byte z of the word
+      return u < 16 ? base + lay.v_codes(h) + (size_t)(ps >> 5) * 2048 + ((ps & 31) >> 3) * 512 + ((u & 3) * 4 + z) * 32 + (u >> 2) * 8 + (ps & 7)
+                    : base + lay.v_scales(h) + (size_t)(ps >> 5) * 128 + ((ps & 31) >> 3) * 32 + z * 8 + (ps & 7);
+    };
+    auto place16 = [&](uint8_t* base, int ps) { return (bf16_t*)base + ((size_t)(ps >> 5) * 128 + u * 2) * 32 + (ps & 31); };
+    if (chunk && e1 - e0 == 8) {
+      uint8_t* base = base_of(slot0);
+      if (KV4) {
+#pragma unroll
+        for (int z = 0; z < 4; ++z) {
+          u32x2 w;
+#pragma unroll
+          for (int d = 0; d < 2; ++d) {
+            const unsigned sel = 0x0c0c0400u + 0x101u * z;                  // byte z of either operand
+            const unsigned ab = __builtin_amdgcn_perm(x[4 * d + 1], x[4 * d], sel), cd = __builtin_amdgcn_perm(x[4 * d + 3], x[4 * d + 2], sel);
+            w[d] = __builtin_amdgcn_perm(cd, ab, 0x05040100u);
+          }
+          st8(place4(base, pos0 + first, z), w);
+        }
+      } else {
+        u32x4 lo, hi;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) { lo[d] = __builtin_amdgcn_perm(x[2 * d + 1], x[2 * d], 0x05040100u); hi[d] = __builtin_amdgcn_perm(x[2 * d + 1], x[2 * d], 0x07060302u); }
+        bf16_t* dst = place16(base, pos0 + first);
+        st16(dst, lo); st16(dst + 32, hi);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {                                         // each row to its own place
+        int sl = chunk ? slot0 : -1, ps = pos0 + first + e;
+        if (e < e0 || e >= e1) continue;
+        if (!chunk) row_place(a, r0 + first + e, sl, ps);
+        if (sl < 0) continue;
+        uint8_t* base = base_of(sl);
+        if (KV4) {
+#pragma unroll
+          for (int z = 0; z < 4; ++z) *place4(base, ps, z) = (uint8_t)(x[e] >> (8 * z));
+        } else {
+          bf16_t* dst = place16(base, ps);
+          dst[0] = (bf16_t)x[e]; dst[32] = (bf16_t)(x[e] >> 16);
+        }
+      }
+    }
+  }
+}
+
+// Eight lanes a (row, head), lane j with channels 8 j .. + 7 and 64 + 8 j .. + 7: the rotation's pairs and, four lanes each, two groups of the 4-bit format
+// (2 shuffles a group, 3 for the norm).  WINDOWS: every v_every-th block takes V of a window of rows, the others queries and keys.
+template <bool KV4, bool WINDOWS>
+__global__ __launch_bounds__(256) void qk_norm_rope_append_kernel(QkNormArgs a, int v_blocks, int v_every) {
+  __shared__ __attribute__((aligned(16))) unsigned char lds[WINDOWS ? 32 * (KV4 ? 68 : 260) : 16];
+  int block = (int)blockIdx.x;
+  if (WINDOWS) {
+    const int w = block / v_every;
+    if (w < v_blocks && block == w * v_every) {
+      const int wins = v_blocks / a.n_kv_heads, h = w / wins;
+      append_v_window<KV4>(a, h, (w - h * wins) * 32, lds);
+      return;
+    }
+    block -= min(w + 1, v_blocks);
+  }
+  const int per_row = a.n_q_heads + (WINDOWS ? 1 : 2) * a.n_kv_heads;
+  // (row, head) of the lane's item 32 block + tid / 8: divided once a block; a row of 32 heads and more ends at most once in a block
+  int s = (block * 32) / per_row, head = block * 32 - s * per_row + (int)(threadIdx.x >> 3);
+  if (per_row >= 32) {
+    if (head >= per_row) { head -= per_row; ++s; }
+  } else {
+    const int more = head / per_row;
+    head -= more * per_row; s += more;
+  }
+  if (s >= a.rows) return;                                                  // whole groups of eight lanes
+  const int j = threadIdx.x & 7, c0 = j * 8, kind = head < a.n_q_heads ? 0 : head < a.n_q_heads + a.n_kv_heads ? 1 : 2;
+  const int h = kind == 0 ? head : head - a.n_q_heads - (kind - 1) * a.n_kv_heads;
+  int slot = 0, pos = 0;
+  if (kind > 0) row_place(a, s, slot, pos);
   u32x4 r1, r2;
   if (kind < 2) {
-    const bf16_t* w = kind == 0 ? a.q_norm : a.k_norm;
-    if (w != nullptr) head_norm(x1, x2, w, c0, a.eps);
+    float x1[8], x2[8];
+    row8(a, s, head * 128 + c0, x1);
+    row8(a, s, head * 128 + 64 + c0, x2);
     const u32x4 cq = ld16(a.cos + (size_t)s * 64 + c0), sq = ld16(a.sin + (size_t)s * 64 + c0);
+    const bf16_t* w = kind ? a.k_norm : a.q_norm;
+    if (w != nullptr) head_norm(x1, x2, w, c0, a.eps);
 #pragma unroll
     for (int d = 0; d < 4; ++d) {
-      float o1[2], o2[2];
+      float p[4], q[4];                                                     // the four products of channels 2 d, 2 d + 1 and their partners, rounded
 #pragma unroll
       for (int z = 0; z < 2; ++z) {
-        const float c = z ? hi2f(cq[d]) : lo2f(cq[d]), sv = z ? hi2f(sq[d]) : lo2f(sq[d]), u = x1[2 * d + z], v = x2[2 * d + z];
-        o1[z] = rbf(u * c) + rbf(-v * sv);
-        o2[z] = rbf(v * c) + rbf(u * sv);
+        const float c = z ? hi2f(cq[d]) : lo2f(cq[d]), sn = z ? hi2f(sq[d]) : lo2f(sq[d]), u = x1[2 * d + z], v = x2[2 * d + z];
+        p[z] = u * c; p[2 + z] = -v * sn;
+        q[z] = v * c; q[2 + z] = u * sn;
       }
-      r1[d] = pack2(o1[0], o1[1]); r2[d] = pack2(o2[0], o2[1]);
+      rbf2(p[0], p[1]); rbf2(p[2], p[3]); rbf2(q[0], q[1]); rbf2(q[2], q[3]);
+      r1[d] = pack2(p[0] + p[2], p[1] + p[3]); r2[d] = pack2(q[0] + q[2], q[1] + q[3]);
     }
     if (kind == 0) {
       bf16_t* q = a.q_out + ((size_t)s * a.n_q_heads + h) * 128 + c0;
       st16(q, r1); st16(q + 64, r2);
       return;
     }
-  } else {
-#pragma unroll
-    for (int d = 0; d < 4; ++d) { r1[d] = pack2(x1[2 * d], x1[2 * d + 1]); r2[d] = pack2(x2[2 * d], x2[2 * d + 1]); }
-  }
-  const int slot = a.tok_stream[s];
-  if (slot < 0 || slot >= a.n_slots) return;                                // a row of no stream
-  const int pos = a.tok_pos != nullptr ? a.tok_pos[s] : a.kv_len[slot];
-  if (pos < 0 || pos >= a.lmax) return;
+  } else row_pairs(a, s, head * 128 + c0, r1, r2);
+  if (slot < 0) return;
   if (!KV4) {
-    const size_t kv = (size_t)a.n_kv_heads * a.lmax * 128;
-    bf16_t* base = (bf16_t*)a.kv_base[slot] + (size_t)a.layer * 2 * kv;
+    bf16_t* base = (bf16_t*)a.kv_base[slot] + ((size_t)(a.layer * 2 + kind - 1) * a.n_kv_heads + h) * a.lmax * 128;
     if (kind == 1) {
-      bf16_t* k = base + ((size_t)h * a.lmax + pos) * 128 + c0;
+      bf16_t* k = base + (size_t)pos * 128 + c0;
       st16(k, r1); st16(k + 64, r2);
     } else {
-      bf16_t* v = base + kv + (size_t)h * a.lmax * 128 + ((size_t)(pos >> 5) * 128 + c0) * 32 + (pos & 31);
+      bf16_t* v = base + ((size_t)(pos >> 5) * 128 + c0) * 32 + (pos & 31);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         v[e * 32] = (bf16_t)((e & 1) ? r1[e >> 1] >> 16 : r1[e >> 1]);
         v[(64 + e) * 32] = (bf16_t)((e & 1) ? r2[e >> 1] >> 16 : r2[e >> 1]);
       }
     }
-  } else {
-    const Kv4Layout lay{a.n_kv_heads, a.lmax};
-    uint8_t* base = (uint8_t*)a.kv_base[slot] + (size_t)a.layer * lay.layer_bytes();
+    return;
+  }
+  const Kv4Layout lay{a.n_kv_heads, a.lmax};
+  uint8_t* base = (uint8_t*)a.kv_base[slot] + (size_t)a.layer * lay.layer_bytes();
+  if (kind == 1) {
     const int e1 = kv4_exponent(max4(max_bits(r1))), e2 = kv4_exponent(max4(max_bits(r2)));       // groups j / 4 and 2 + j / 4
-    const unsigned w1 = fp4_of(r1, e1), w2 = fp4_of(r2, e2);
-    if (kind == 1) {
-      unsigned* k = (unsigned*)(base + lay.k_codes(h) + (size_t)pos * 64);
-      k[j] = w1; k[8 + j] = w2;
-      if ((j & 3) == 0) {
-        uint8_t* sc = base + lay.k_scales(h) + (size_t)pos * 4;
-        sc[j >> 2] = (uint8_t)e1; sc[2 + (j >> 2)] = (uint8_t)e2;
-      }
-    } else {
-      // channels i and 16 + i of a group lie two lanes apart: the lower pair of lanes takes the lower group's bytes, the upper pair the upper group's
-      const bool up = (j & 2) != 0;
-      const unsigned mine = up ? w2 : w1, other = __shfl_xor(up ? w1 : w2, 2, 64);
-      const unsigned lo = up ? other : mine, hi = up ? mine : other;
-      const int t = up ? 2 + (j >> 2) : j >> 2;
-      uint8_t* v = base + lay.v_codes(h) + (size_t)(pos >> 5) * 2048 + ((pos & 31) >> 3) * 512 + (j & 1) * 256 + t * 8 + (pos & 7);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e * 32] = (uint8_t)((lo >> (4 * e) & 15) | (hi >> (4 * e) & 15) << 4);
-      if ((j & 1) == 0) base[lay.v_scales(h) + (size_t)(pos >> 5) * 128 + ((pos & 31) >> 3) * 32 + t * 8 + (pos & 7)] = (uint8_t)(up ? e2 : e1);
+    unsigned* k = (unsigned*)(base + lay.k_codes(h) + (size_t)pos * 64);
+    k[j] = fp4_of(r1, e1); k[8 + j] = fp4_of(r2, e2);
+    if ((j & 3) == 0) {
+      uint8_t* sc = base + lay.k_scales(h) + (size_t)pos * 4;
+      sc[j >> 2] = (uint8_t)e1; sc[2 + (j >> 2)] = (uint8_t)e2;
     }
+  } else {
+    u32x2 b; int t, e;
+    v_codes(r1, r2, j, b, t, e);
+    uint8_t* v = base + lay.v_codes(h) + (size_t)(pos >> 5) * 2048 + ((pos & 31) >> 3) * 512 + (j & 1) * 256 + t * 8 + (pos & 7);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i * 32] = (uint8_t)(b[i >> 2] >> (8 * (i & 3)));
+    if ((j & 1) == 0) base[lay.v_scales(h) + (size_t)(pos >> 5) * 128 + ((pos & 31) >> 3) * 32 + t * 8 + (pos & 7)] = (uint8_t)e;
   }
 }
 
@@ -240,10 +371,16 @@ static int qk_norm_check(const QkNormArgs& a) {
 int qk_norm_rope_append(const QkNormArgs& a, bool kv4, hipStream_t st) {
   if (int rc = qk_norm_check(a)) return rc;
   if (a.rows == 0) return 0;
-  const int64_t blocks = ((int64_t)a.rows * (a.n_q_heads + 2 * a.n_kv_heads) + 31) / 32;
-  if (blocks > 0x7fffffff) return LCC_ERR_SHAPE;
-  if (kv4) qk_norm_rope_append_kernel<true><<<dim3((unsigned)blocks), dim3(256), 0, st>>>(a);
-  else qk_norm_rope_append_kernel<false><<<dim3((unsigned)blocks), dim3(256), 0, st>>>(a);
+  const bool windows = a.rows >= KV4_WINDOW_ROWS;
+  const int64_t items = (int64_t)a.rows * (a.n_q_heads + (windows ? 1 : 2) * a.n_kv_heads), blocks = (items + 31) / 32;
+  const int64_t v_blocks = windows ? ((int64_t)a.rows + 31) / 32 * a.n_kv_heads : 0;
+  if (items > 0x7fffff00 || blocks + v_blocks > 0x7fffffff) return LCC_ERR_SHAPE;
+  const dim3 grid((unsigned)(blocks + v_blocks));
+  const int every = windows ? (int)(((blocks + v_blocks) / v_blocks - 1) | 1) : 1;         // V blocks among the others, an odd number apart: blocks go round the eight XCDs
+  if (windows && kv4) qk_norm_rope_append_kernel<true, true><<<grid, dim3(256), 0, st>>>(a, (int)v_blocks, every);
+  else if (windows) qk_norm_rope_append_kernel<false, true><<<grid, dim3(256), 0, st>>>(a, (int)v_blocks, every);
+  else if (kv4) qk_norm_rope_append_kernel<true, false><<<grid, dim3(256), 0, st>>>(a, 0, 1);
+  else qk_norm_rope_append_kernel<false, false><<<grid, dim3(256), 0, st>>>(a, 0, 1);
   return 0;
 }
 

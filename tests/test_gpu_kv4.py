@@ -145,6 +145,44 @@ def test_append_at_kv_len_and_rows_of_no_stream(dev, bits):
         assert not held.any() and (slot in (0, 2) or not kv.buf[slot].any())
 
 
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("rows", [130, 600])
+@pytest.mark.parametrize("how", ["tokens of many streams", "a chunk with gaps", "one chunk", "two chunks", "a chunk that leaves the arena"])
+def test_append_of_many_rows(dev, bits, rows, how):
+    """from 512 rows on V goes by windows of 32 rows, whole runs of eight positions where a window is one chunk, rows one by one where it is not"""
+    from livecc_amd import ops
+    heads, kv_heads, lmax = 2, 2, 640
+    if how == "tokens of many streams":
+        n, lmax, lens = rows, 32, [(37 * s) % 32 for s in range(rows)]
+        stream = list(reversed(range(rows)))
+        pos = [lens[s] for s in stream]
+    else:
+        n, lens = 2, [0, 0]
+        first = {"a chunk with gaps": 21, "a chunk that leaves the arena": lmax - rows + 3}.get(how, 5)
+        stream, pos = [1] * rows, [first + r for r in range(rows)]
+        if how == "a chunk with gaps":
+            stream[40], pos[75], pos[76] = -1, lmax - 1, -2
+        if how == "two chunks":
+            stream[77:], pos[77:] = [0] * (rows - 77), list(range(rows - 77))
+    S = rows
+    qkv = rand((S, 6 * 128), dev, 6)
+    cos, sin = tables(pos, dev)
+    kv = (ops.Kv4Arena if bits == 4 else ops.KvArena)(n, 2, kv_heads, lmax, dev)
+    by_len = how == "tokens of many streams"
+    ops.qk_norm_rope_kv_append(qkv, cos, sin, i32(stream, dev), None if by_len else i32(pos, dev), kv, 1, heads, kv_len=i32(lens, dev) if by_len else None)
+    x = qkv.cpu().view(S, 6, 128)
+    want = [U.norm_rope(x[:, 2:4], None, cos.cpu(), sin.cpu()), x[:, 4:].double()]
+    want = [U.quantise(w)[2] for w in want] if bits == 4 else want
+    for view, w in ((kv.k_view, want[0]), (kv.v_view, want[1])):
+        held = torch.stack([view(s, 1) for s in range(n)]).double().cpu()
+        for i, (s, p) in enumerate(zip(stream, pos)):
+            if s >= 0 and 0 <= p < lmax:
+                assert torch.equal(held[s, :, p], w[i]), (s, p)
+                held[s, :, p] = 0
+        assert not held.any()
+    assert not kv.buf[:, :kv.buf.shape[1] // 2].any()
+
+
 def test_codes_of_every_bf16(dev):
     """Groups whose largest magnitude is each of the finite bf16 magnitudes in turn, beside values spread over its binades, zeros, and both signs; infinities and NaN."""
     from livecc_amd import ops
