@@ -394,23 +394,25 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4Args a, const int32_t*
   if (item >= (int64_t)rows * a.n_kv_heads) return;
   const int s = (int)(item / a.n_kv_heads), h = (int)(item - (int64_t)s * a.n_kv_heads), j = threadIdx.x & 7;
   const int slot = tok_stream[s], pos = tok_pos[s];
-  bf16_t *ko = k_out + (size_t)item * 128 + j * 16, *vo = v_out + (size_t)item * 128 + j * 16;
+  // K: channels 16 j .. + 15.  V: bytes i = 8 z .. + 7 of group t, that is channels 32 t + 8 z .. + 7 and 32 t + 16 + 8 z .. + 7
+  const int t = j >> 1, z = j & 1;
+  bf16_t *ko = k_out + (size_t)item * 128 + j * 16, *vo = v_out + (size_t)item * 128 + t * 32 + z * 8;
   u32x4 k0 = {0, 0, 0, 0}, k1 = k0, v0 = k0, v1 = k0;
   if (slot >= 0 && slot < a.n_slots && pos >= 0 && pos < a.lmax) {
     const Kv4Layout lay{a.n_kv_heads, a.lmax};
     const uint8_t* base = (const uint8_t*)a.kv_base[slot] + (size_t)a.layer * lay.layer_bytes();
     const u32x2 kc = ld8(base + lay.k_codes(h) + (size_t)pos * 64 + j * 8);
-    const unsigned ks = (unsigned)base[lay.k_scales(h) + (size_t)pos * 4 + (j >> 1)] << 23;
-    k0 = fp4_word(kc[0], ks); k1 = fp4_word(kc[1], ks);
-    const int t = j >> 1, sh = (j & 1) * 4, g = (pos & 31) >> 3, e = pos & 7;
-    const uint8_t* vc = base + lay.v_codes(h) + (size_t)(pos >> 5) * 2048 + g * 512 + t * 8 + e;
+    const unsigned ks = (unsigned)base[lay.k_scales(h) + (size_t)pos * 4 + t] << 23;
+    const int g = (pos & 31) >> 3, e = pos & 7;
+    const uint8_t* vc = base + lay.v_codes(h) + (size_t)(pos >> 5) * 2048 + g * 512 + z * 256 + t * 8 + e;
     const unsigned vs = (unsigned)base[lay.v_scales(h) + (size_t)(pos >> 5) * 128 + g * 32 + t * 8 + e] << 23;
-    unsigned w[2] = {0, 0};
+    unsigned lo = 0, hi = 0;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) w[i >> 3] |= (unsigned)(vc[i * 32] >> sh & 15) << (4 * (i & 7));
-    v0 = fp4_word(w[0], vs); v1 = fp4_word(w[1], vs);
+    for (int i = 0; i < 8; ++i) { const unsigned b = vc[i * 32]; lo |= (b & 15u) << (4 * i); hi |= (b >> 4) << (4 * i); }
+    k0 = fp4_word(kc[0], ks); k1 = fp4_word(kc[1], ks);
+    v0 = fp4_word(lo, vs); v1 = fp4_word(hi, vs);
   }
-  st16(ko, k0); st16(ko + 8, k1); st16(vo, v0); st16(vo + 8, v1);
+  st16(ko, k0); st16(ko + 8, k1); st16(vo, v0); st16(vo + 16, v1);
 }
 int kv4_read(const Kv4Args& a, const int32_t* tok_stream, const int32_t* tok_pos, bf16_t* k, bf16_t* v, int rows, hipStream_t st) {
   if (int rc = a.check()) return rc;
@@ -445,19 +447,25 @@ LCC_DEVICE void kv4_load_v(Kv4Tile& t, const Kv4Head& h, int blk, unsigned li, u
   t.s[0] = ld16(vs + g * 32); t.s[1] = ld16(vs + (g * 32 + 16));
 }
 
-template <int NW>
-__global__ __launch_bounds__(NW * 64, 4) void attn_decode_kv4_kernel(Kv4Args a, const bf16_t* __restrict__ q, const int32_t* __restrict__ slots,
-                                                                     const int32_t* __restrict__ kv_len, int n_q_heads, int nsplit,
-                                                                     float* __restrict__ ws_o, float* __restrict__ ws_ml, bf16_t* __restrict__ out, float scale_log2e) {
+// What the columns are: rows of a decode step (row b alone, its slot's length), or (CHUNK) a tile of a few rows of a stream.
+struct Kv4Rows { const int32_t* slot; const int32_t* kv_len; const int32_t* q0; const int32_t* nq; const int32_t* pos0; int tile_rows, n_rows; };
+
+template <int NW, bool CHUNK>
+__global__ __launch_bounds__(NW * 64, 4) void attn_rows_kv4_kernel(Kv4Args a, Kv4Rows rows, const bf16_t* __restrict__ q, int n_q_heads, int nsplit, float* __restrict__ ws_o,
+                                                                   float* __restrict__ ws_ml, bf16_t* __restrict__ out, float scale_log2e) {
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   float (*mo)[16][132] = reinterpret_cast<float (*)[16][132]>(lds);
   __shared__ float mm[NW][16], ml[NW][16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, g = lane >> 4;
   const int split = blockIdx.x, hk = blockIdx.y, b = blockIdx.z, G = n_q_heads / a.n_kv_heads;
-  const int slot = slots[b];
+  const int slot = rows.slot[b];
   const bool live = slot >= 0 && slot < a.n_slots;
-  const int n = live ? max(0, min(kv_len[slot], a.lmax - 1) + 1) : 0;       // keys (a length below zero: none)
+  const int q0 = CHUNK ? rows.q0[b] : b, nq = CHUNK ? min(min(rows.nq[b], rows.tile_rows), rows.n_rows - q0) : 1;
+  if (CHUNK && (q0 < 0 || nq <= 0)) return;
+  const int pos0 = !live ? -1 : CHUNK ? min(rows.pos0[b], a.lmax) : min(rows.kv_len[slot], a.lmax - 1);       // of the first row
+  const int n = live ? max(0, min(pos0 + nq, a.lmax)) : 0;                  // keys (a position below zero: none)
   const int nblk = (n + 31) >> 5, per = (nblk + nsplit - 1) / nsplit, b0 = split * per, b1 = min(nblk, b0 + per);
+  const int r = CHUNK ? li / G : 0, lim = live ? pos0 + min(r, nq - 1) : -1;                                  // the column's row and the last key it sees
 
   f32x4 o[8];
 #pragma unroll
@@ -470,7 +478,7 @@ __global__ __launch_bounds__(NW * 64, 4) void attn_decode_kv4_kernel(Kv4Args a, 
     const Kv4Head head{base + lay.k_codes(hk), base + lay.v_codes(hk), base + lay.k_scales(hk), base + lay.v_scales(hk)};
     const unsigned key = 8 * (li >> 2) + (li & 3);
     u32x4 qf[4];
-    const bf16_t* qp = q + ((size_t)b * n_q_heads + hk * G + min(li, G - 1)) * 128 + g * 32;
+    const bf16_t* qp = q + ((size_t)(q0 + min(r, nq - 1)) * n_q_heads + hk * G + (CHUNK ? li - r * G : min(li, G - 1))) * 128 + g * 32;
 #pragma unroll
     for (int s = 0; s < 4; ++s) qf[s] = ld16(qp + 8 * s);
     Kv4Tile cur;
@@ -488,29 +496,51 @@ __global__ __launch_bounds__(NW * 64, 4) void attn_decode_kv4_kernel(Kv4Args a, 
         for (int s = 0; s < 4; ++s) sc[T] = mfma16(as_bf16x8(fp4_word(cur.k[T][s], cur.ks[T] << 23)), as_bf16x8(qf[s]), sc[T]);
       }
       kv4_load_k(cur, head, nb, key, g);                                    // into the registers that the products have left
-      const int left = n - blk * 32 - 8 * g;                                // keys of this lane's octet that exist
-      if (n - blk * 32 < 32) {                                              // the last block: scores of no key to -inf, V there to zero (0 * NaN)
+      bool nan[4] = {false, false, false, false};                           // CHUNK: the column sees a V of this group that is NaN
+      if (blk * 32 + 31 > pos0) {                                           // some column does not see all of the block: scores of its hidden keys to -inf
+        const int key0 = blk * 32 + 8 * g, left = n - key0;                 // of this lane's octet; keys that exist
 #pragma unroll
         for (int T = 0; T < 2; ++T)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) sc[T][r] = 4 * T + r < left ? sc[T][r] : -INFINITY;
+          for (int e = 0; e < 4; ++e) sc[T][e] = key0 + 4 * T + e <= lim ? sc[T][e] : -INFINITY;
+        // V of no key to zero (0 * NaN), and NaN values that a row before theirs must not meet: zero here, put behind the products into the columns that see them
         const unsigned long long keep = left >= 8 ? ~0ull : left <= 0 ? 0ull : (1ull << (8 * left)) - 1;
 #pragma unroll
-        for (int t = 0; t < 2; ++t) { cur.s[t][0] &= (unsigned)keep; cur.s[t][1] &= (unsigned)(keep >> 32); cur.s[t][2] &= (unsigned)keep; cur.s[t][3] &= (unsigned)(keep >> 32); }
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int z = 0; z < 2; ++z) {
+            const unsigned w = cur.s[t >> 1][2 * (t & 1) + z] & (unsigned)(keep >> (32 * z));
+            if (CHUNK) {
+              const unsigned bad = ((w & 0x7f7f7f7fu) + 0x03030303u) & w & 0x80808080u;      // bytes of 253 and more
+              const int seen = lim - key0 - 4 * z;                          // bytes 0 .. seen
+              nan[t] |= (bad & (seen >= 3 ? ~0u : seen < 0 ? 0u : (256u << (8 * seen)) - 1)) != 0;
+              cur.s[t >> 1][2 * (t & 1) + z] = w & ~((bad >> 7) * 255u);
+            } else cur.s[t >> 1][2 * (t & 1) + z] = w;
+          }
+        if (CHUNK) {
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {                                     // over the four octets
+            int any = nan[t];
+            any |= __shfl_xor(any, 16, 64);
+            any |= __shfl_xor(any, 32, 64);
+            nan[t] = any != 0;
+          }
+        }
       }
       float top = __builtin_fmaxf(__builtin_fmaxf(__builtin_fmaxf(sc[0][0], sc[0][1]), __builtin_fmaxf(sc[0][2], sc[0][3])),
                                   __builtin_fmaxf(__builtin_fmaxf(sc[1][0], sc[1][1]), __builtin_fmaxf(sc[1][2], sc[1][3])));
       top = xor32_max(xor16_max(top)) * scale_log2e;
       if (__any(top > m + KV4_SLACK)) {
-        const float mn = __builtin_fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - mn);
+        const float mn = __builtin_fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
         l *= f;
 #pragma unroll
         for (int t = 0; t < 8; ++t) o[t] *= f;
         m = mn;
       }
+      const float mu = CHUNK && m == -INFINITY ? 0.f : m;                   // a column that has seen no key
       float p[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) { p[e] = __builtin_amdgcn_exp2f(fmaf(sc[e >> 2][e & 3], scale_log2e, -m)); l += p[e]; }
+      for (int e = 0; e < 8; ++e) { p[e] = __builtin_amdgcn_exp2f(fmaf(sc[e >> 2][e & 3], scale_log2e, -mu)); l += p[e]; }
       // A converted byte is a pair (channel i, channel 16 + i) of one key, two slots of the operand: against (p, 0) it is channel i's product, against (0, p) the other's.
       u32x4 pl[2], ph[2];
 #pragma unroll
@@ -524,6 +554,11 @@ __global__ __launch_bounds__(NW * 64, 4) void attn_decode_kv4_kernel(Kv4Args a, 
           o[2 * t] = mfma16(v, as_bf16x8(pl[z]), o[2 * t]);
           o[2 * t + 1] = mfma16(v, as_bf16x8(ph[z]), o[2 * t + 1]);
         }
+      if (CHUNK) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          if (nan[t]) { o[2 * t] = (f32x4){NAN, NAN, NAN, NAN}; o[2 * t + 1] = o[2 * t]; }
+      }
       kv4_load_v(cur, head, nb, li, g);
       asm volatile("" ::: "memory");           // hipcc would move the loads to the head of the next turn, in front of their wait
     }
@@ -534,8 +569,8 @@ __global__ __launch_bounds__(NW * 64, 4) void attn_decode_kv4_kernel(Kv4Args a, 
   for (int t = 0; t < 8; ++t) *reinterpret_cast<f32x4*>(&mo[wave][li][16 * t + 4 * g]) = o[t];
   if (g == 0) { mm[wave][li] = m; ml[wave][li] = l; }
   __syncthreads();
-  for (int i = threadIdx.x; i < G * 32; i += NW * 64) {
-    const int h = i >> 5, c = (i & 31) * 4;
+  for (int i = threadIdx.x; i < nq * G * 32; i += NW * 64) {
+    const int h = i >> 5, c = (i & 31) * 4;                                  // column, channel
     float M = -INFINITY, L = 0.f;
 #pragma unroll
     for (int w = 0; w < NW; ++w) M = __builtin_fmaxf(M, mm[w][h]);
@@ -547,7 +582,8 @@ __global__ __launch_bounds__(NW * 64, 4) void attn_decode_kv4_kernel(Kv4Args a, 
       L += f * ml[w][h];
       acc += f * *reinterpret_cast<const f32x4*>(&mo[w][h][c]);
     }
-    const size_t row = (size_t)b * n_q_heads + hk * G + h;
+    const int rr = CHUNK ? h / G : 0;
+    const size_t row = (size_t)(q0 + rr) * n_q_heads + hk * G + (h - rr * G);
     if (nsplit == 1) {
       const float r = L == 0.f ? 0.f : 1.f / L;
       st8(out + row * 128 + c, (u32x2){pack2(acc[0] * r, acc[1] * r), pack2(acc[2] * r, acc[3] * r)});
@@ -612,6 +648,18 @@ int kv4_decode_splits(const int32_t* n_keys, int n, int n_kv_heads) {
   return (int)std::max(k, 1L);
 }
 
+// eight waves where a block has all keys, four where they are split: 16 waves a unit in either case once there are blocks enough
+template <bool CHUNK>
+static void attn_rows_launch(const Kv4Args& a, const Kv4Rows& rows, int n, const bf16_t* q, int n_q_heads, int nsplit, float* ws_o, float* ws_ml, bf16_t* out, hipStream_t st) {
+  static DeviceOnce once;
+  constexpr int part = 16 * 132 * 4;                                        // LDS of a wave's result
+  if (once.first()) (void)hipFuncSetAttribute((const void*)attn_rows_kv4_kernel<8, CHUNK>, hipFuncAttributeMaxDynamicSharedMemorySize, 8 * part);
+  const dim3 grid(nsplit, a.n_kv_heads, n);
+  const float scale = 1.4426950408889634f / sqrtf(128.f);
+  if (nsplit == 1) attn_rows_kv4_kernel<8, CHUNK><<<grid, dim3(512), 8 * part, st>>>(a, rows, q, n_q_heads, nsplit, ws_o, ws_ml, out, scale);
+  else attn_rows_kv4_kernel<4, CHUNK><<<grid, dim3(256), 4 * part, st>>>(a, rows, q, n_q_heads, nsplit, ws_o, ws_ml, out, scale);
+}
+
 int attn_decode_kv4(const Kv4Args& a, const bf16_t* q, const int32_t* slots, const int32_t* kv_len, int rows, int n_q_heads, int nsplit, float* ws_o, float* ws_ml,
                     bf16_t* out, hipStream_t st) {
   if (int rc = a.check()) return rc;
@@ -619,13 +667,7 @@ int attn_decode_kv4(const Kv4Args& a, const bf16_t* q, const int32_t* slots, con
     return LCC_ERR_SHAPE;
   if (nsplit > 1 && (ws_o == nullptr || ws_ml == nullptr)) return LCC_ERR_ARG;
   if (rows == 0) return 0;
-  static DeviceOnce once;
-  constexpr int part = 16 * 132 * 4;                                        // LDS of a wave's result
-  if (once.first()) (void)hipFuncSetAttribute((const void*)attn_decode_kv4_kernel<8>, hipFuncAttributeMaxDynamicSharedMemorySize, 8 * part);
-  const dim3 grid(nsplit, a.n_kv_heads, rows);
-  const float scale = 1.4426950408889634f / sqrtf(128.f);
-  if (nsplit == 1) attn_decode_kv4_kernel<8><<<grid, dim3(512), 8 * part, st>>>(a, q, slots, kv_len, n_q_heads, nsplit, ws_o, ws_ml, out, scale);
-  else attn_decode_kv4_kernel<4><<<grid, dim3(256), 4 * part, st>>>(a, q, slots, kv_len, n_q_heads, nsplit, ws_o, ws_ml, out, scale);
+  attn_rows_launch<false>(a, Kv4Rows{slots, kv_len, nullptr, nullptr, nullptr, 1, rows}, rows, q, n_q_heads, nsplit, ws_o, ws_ml, out, st);
   if (nsplit > 1) kv4_combine(ws_o, ws_ml, out, (int64_t)rows * n_q_heads, nsplit, st);
   return 0;
 }
@@ -639,7 +681,7 @@ constexpr int KV4_STAGE = 64, KV4_KB = KV4_STAGE * 256, KV4_VB = 128 * KV4_STAGE
 template <int U> struct Kv4Stage { u32x2 k[U], v[U], s[U]; unsigned ks[U]; };
 
 template <int NW>
-__global__ __launch_bounds__(NW * 64, 2) void attn_prefill_kv4_kernel(Kv4Args a, const bf16_t* __restrict__ q, bf16_t* __restrict__ out, const int32_t* __restrict__ tile_stream,
+__global__ __launch_bounds__(NW * 64, 2) void attn_chunk_kv4_kernel(Kv4Args a, const bf16_t* __restrict__ q, bf16_t* __restrict__ out, const int32_t* __restrict__ tile_stream,
                                                                       const int32_t* __restrict__ tile_q0, const int32_t* __restrict__ tile_nq,
                                                                       const int32_t* __restrict__ tile_pos0, int n_q_heads, int tile_rows, int nsplit, int n_rows,
                                                                       float* __restrict__ ws_o, float* __restrict__ ws_ml, float scale_log2e) {
@@ -852,52 +894,79 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_prefill_kv4_kernel(Kv4Args a,
     if (masked(top_st)) put_nan(top_st);
     l = xor32_sum(l);
   }
-  if (!valid) return;
-  const size_t row = (size_t)(q0 + r) * n_q_heads + hk * G + h;
-  if (nsplit == 1) {
-    const float f = l == 0.f ? 0.f : 1.f / l;
+  // The result goes through LDS, a wave by itself, 32 columns x 64 channels at a time (16-byte chunks permuted by the column): a store is then of four columns' 256 bytes.
+  // Straight from the registers, 32 bytes of a column at a time, the partials of 17 rows in 64 splits took 9 us of 21.
+  const float f = nsplit > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+  const int mine = valid ? (q0 + r) * n_q_heads + hk * G + h : -1;
+  if (nsplit > 1 && valid && hh == 0) { ws_ml[((size_t)mine * nsplit + split) * 2] = m; ws_ml[((size_t)mine * nsplit + split) * 2 + 1] = l; }
+  __syncthreads();                                                          // every wave has read its operands
+  unsigned char* tr = lds + wave * 8192;
 #pragma unroll
-    for (int d = 0; d < 4; ++d)
+  for (int half = 0; half < 2; ++half) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        st8(out + row * 128 + d * 32 + 8 * i + 4 * hh, (u32x2){pack2(o[d][4 * i] * f, o[d][4 * i + 1] * f), pack2(o[d][4 * i + 2] * f, o[d][4 * i + 3] * f)});
-  } else {
-    float* w = ws_o + (row * nsplit + split) * 128;
+    for (int d = 0; d < 2; ++d)
 #pragma unroll
-    for (int d = 0; d < 4; ++d)
+      for (int i = 0; i < 4; ++i) {
+        const f32x16& v = o[2 * half + d];
+        *reinterpret_cast<f32x4*>(tr + col * 256 + (((d * 8 + 2 * i + hh) ^ (col & 15)) << 4)) = (f32x4){v[4 * i] * f, v[4 * i + 1] * f, v[4 * i + 2] * f, v[4 * i + 3] * f};
+      }
+    wave_lds_order();
 #pragma unroll
-      for (int i = 0; i < 4; ++i) *reinterpret_cast<f32x4*>(w + d * 32 + 8 * i + 4 * hh) = (f32x4){o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
-    if (hh == 0) { ws_ml[(row * nsplit + split) * 2] = m; ws_ml[(row * nsplit + split) * 2 + 1] = l; }
+    for (int it = 0; it < 8; ++it) {
+      const int cc = it * 4 + (lane >> 4), row = __shfl(mine, cc, 64), ch = half * 64 + (lane & 15) * 4;
+      const f32x4 v = *reinterpret_cast<const f32x4*>(tr + cc * 256 + (((lane & 15) ^ (cc & 15)) << 4));
+      if (row < 0) continue;
+      if (nsplit > 1) *reinterpret_cast<f32x4*>(ws_o + ((size_t)row * nsplit + split) * 128 + ch) = v;
+      else st8(out + (size_t)row * 128 + ch, (u32x2){pack2(v[0], v[1]), pack2(v[2], v[3])});
+    }
+    wave_lds_order();
   }
 }
 
-// Tile height and key splits.  Blocks of eight waves (256 columns), one a compute unit; where no stream has more than 128 columns, of four waves, two a unit.  Cost in
-// stages of 64 keys (1.6 us in either): a block's prologue and result count as 2.5; blocks that all run at once take as long as the longest, more of them the mean
-// plus most of one; the join costs a launch (2 stages) and its partials written and read (1,040 bytes a row, head and split at 4.5 TB/s).
+// Tile height -- which of the three kernels -- and key splits, by a cost in us.  All: 4 for the launch and the way to the first key; splits another launch (3) and their
+// partials, 1,040 bytes a row, head and split written and read at 4.5 TB/s.
+//   16 columns (attn_rows_kv4_kernel): a wave's 32-key block takes 1.1 when waves are few and 0.75 of a SIMD's time when they are many.
+//   128 or 256 columns (attn_chunk_kv4_kernel of four waves, two blocks a unit, or eight): a stage of 64 keys 1.6 (four waves: alone on a unit 1.2, two blocks 1.8), a block's prologue
+//   and result as 2.5 stages; blocks
+//   that all run at once take as long as the longest, more of them the mean and most of one.
+// Measured, 16 / 128 columns (us): 28 / 4 heads on 26,000 keys 2 rows 11.8 / 20.3, 8 rows 17.3 / 23.5, 12 rows 22.5 / 25.3, 18 rows 29.6 / 27.2; 18 rows on 500 keys of
+// 64 / 8 heads 7.9 / 15.8; 8 x 18 rows on 3,000 keys 30.3 / 27.7.  128 / 256 columns: 8 x ~340 rows on ~5,000 keys 266 / 263, 386 rows on 6,100 60 / 56.
 int kv4_prefill_plan(const int32_t* n_new, const int32_t* past, int n, int n_q_heads, int n_kv_heads, int cus, int* tile_rows, int* nsplit) {
   if (n < 0 || n_q_heads < 1 || n_kv_heads < 1 || n_q_heads % n_kv_heads || n_q_heads / n_kv_heads > 16 || cus < 1) return LCC_ERR_SHAPE;
   const int G = n_q_heads / n_kv_heads;
-  long most = 0, rows = 0;
+  long rows = 0;
   for (int i = 0; i < n; ++i) {
     if (n_new[i] < 0 || past[i] < 0) return LCC_ERR_SHAPE;
-    most = std::max(most, (long)n_new[i]);
     rows += n_new[i];
   }
-  const bool small = most * G <= 128;
-  const int height = (small ? 128 : 256) / G;
-  long tiles = 0, total = 0, longest = 0;
-  for (int i = 0; i < n; ++i)
-    for (long r = 0; r < n_new[i]; r += height) {
-      const long st = (past[i] + std::min<long>(n_new[i], r + height) + KV4_STAGE - 1) / KV4_STAGE;
-      ++tiles; total += st; longest = std::max(longest, st);
-    }
-  const float slots = (float)cus * (small ? 2 : 1), join = rows * (float)n_q_heads * (1040.f / 4.5e6f / 1.6f);
-  *tile_rows = height; *nsplit = 1;
+  const float join = rows * (float)n_q_heads * (1040.f / 4.5e6f);
   float best = 1e30f;
-  for (int k = 1; k <= 64 && k <= std::max(1L, longest / 4); ++k) {
-    const float block = (float)longest / k + 2.5f, blocks = (float)tiles * n_kv_heads * k;
-    const float cost = (blocks <= slots ? block : (total * (float)n_kv_heads + 2.5f * blocks) / slots + 0.8f * block) + (k > 1 ? 2.f + join * k : 0.f);
-    if (cost < best) { best = cost; *nsplit = k; }
+  *tile_rows = 256 / G; *nsplit = 1;
+  for (const int columns : {16, 128, 256}) {
+    const int height = columns / G, keys = columns == 16 ? 32 : KV4_STAGE;
+    long tiles = 0, total = 0, longest = 0;                                 // stages (blocks of 32 keys) of a KV head
+    for (int i = 0; i < n; ++i) {
+      const long count = (n_new[i] + height - 1) / height;
+      tiles += count;
+      for (long z = 0; z < std::min(count, 64L); ++z) {                     // of many tiles 64 spread over the stream stand for all
+        const long t = count <= 64 ? z : z * count / 64, st = (past[i] + std::min<long>(n_new[i], (t + 1) * height) + keys - 1) / keys;
+        total += count <= 64 ? st : st * count / 64;
+        longest = std::max(longest, st);
+      }
+    }
+    if (tiles > 65535) continue;
+    for (int k = 1; k <= 64 && k <= std::max(1L, longest / 4); ++k) {
+      const float blocks = (float)tiles * n_kv_heads * k, work = (float)total * n_kv_heads;
+      float cost = 4.f + (k > 1 ? 3.f + join * k : 0.f);
+      if (columns == 16) {
+        const float one = 1.1f * (float)((longest + (k == 1 ? 8 : 4) * k - 1) / ((k == 1 ? 8 : 4) * k)), all = work * 0.75f / (4.f * cus);
+        cost += std::max(one, all + (blocks > cus ? 0.5f * one : 0.f));
+      } else {
+        const float slots = (float)cus * (columns == 128 ? 2 : 1), block = (float)longest / k + 2.5f;
+        cost += blocks <= slots ? (columns == 256 ? 1.6f : blocks <= cus ? 1.2f : 1.8f) * block : 1.6f * ((work + 2.5f * blocks) / slots * (columns == 128 ? 1.5f : 1.f) + 0.8f * block);
+      }
+      if (cost < best) { best = cost; *tile_rows = height; *nsplit = k; }
+    }
   }
   return 0;
 }
@@ -912,15 +981,17 @@ int attn_prefill_kv4(const Kv4Args& a, const bf16_t* q, bf16_t* out, const int32
   if (n_tiles == 0 || n_rows == 0) return 0;
   static DeviceOnce once;
   if (once.first()) {
-    (void)hipFuncSetAttribute((const void*)attn_prefill_kv4_kernel<8>, hipFuncAttributeMaxDynamicSharedMemorySize, KV4_LDS);
-    (void)hipFuncSetAttribute((const void*)attn_prefill_kv4_kernel<4>, hipFuncAttributeMaxDynamicSharedMemorySize, KV4_LDS);
+    (void)hipFuncSetAttribute((const void*)attn_chunk_kv4_kernel<8>, hipFuncAttributeMaxDynamicSharedMemorySize, KV4_LDS);
+    (void)hipFuncSetAttribute((const void*)attn_chunk_kv4_kernel<4>, hipFuncAttributeMaxDynamicSharedMemorySize, KV4_LDS);
   }
   const dim3 grid(a.n_kv_heads, n_tiles, nsplit);
   const float scale = 1.4426950408889634f / sqrtf(128.f);
-  if (tile_rows * (n_q_heads / a.n_kv_heads) > 128)
-    attn_prefill_kv4_kernel<8><<<grid, dim3(512), KV4_LDS, st>>>(a, q, out, tile_stream, tile_q0, tile_nq, tile_pos0, n_q_heads, tile_rows, nsplit, n_rows, ws_o, ws_ml, scale);
+  if (tile_rows * (n_q_heads / a.n_kv_heads) <= 16)
+    attn_rows_launch<true>(a, Kv4Rows{tile_stream, nullptr, tile_q0, tile_nq, tile_pos0, tile_rows, n_rows}, n_tiles, q, n_q_heads, nsplit, ws_o, ws_ml, out, st);
+  else if (tile_rows * (n_q_heads / a.n_kv_heads) > 128)
+    attn_chunk_kv4_kernel<8><<<grid, dim3(512), KV4_LDS, st>>>(a, q, out, tile_stream, tile_q0, tile_nq, tile_pos0, n_q_heads, tile_rows, nsplit, n_rows, ws_o, ws_ml, scale);
   else
-    attn_prefill_kv4_kernel<4><<<grid, dim3(256), KV4_LDS, st>>>(a, q, out, tile_stream, tile_q0, tile_nq, tile_pos0, n_q_heads, tile_rows, nsplit, n_rows, ws_o, ws_ml, scale);
+    attn_chunk_kv4_kernel<4><<<grid, dim3(256), KV4_LDS, st>>>(a, q, out, tile_stream, tile_q0, tile_nq, tile_pos0, n_q_heads, tile_rows, nsplit, n_rows, ws_o, ws_ml, scale);
   if (nsplit > 1) kv4_combine(ws_o, ws_ml, out, (int64_t)n_rows * n_q_heads, nsplit, st);
   return 0;
 }

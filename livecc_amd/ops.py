@@ -572,7 +572,7 @@ def attn_decode4(q: torch.Tensor, kv: Kv4Arena, layer: int, slots: torch.Tensor,
 class Kv4PrefillPlan:
     """Launch plan of `attn_prefill4`: made once for a call's segments, used for every layer."""
 
-    def __init__(self, segments: Sequence[Tuple[int, int, int]], n_q_heads: int, n_kv_heads: int, device, nsplit: int = 0):
+    def __init__(self, segments: Sequence[Tuple[int, int, int]], n_q_heads: int, n_kv_heads: int, device, nsplit: int = 0, tile_rows: int = 0):
         seg = np.asarray(list(segments), dtype=np.int32).reshape(-1, 3)
         new, past = np.ascontiguousarray(seg[:, 1]), np.ascontiguousarray(seg[:, 2])
         device = torch.device(device)
@@ -580,7 +580,7 @@ class Kv4PrefillPlan:
         plan = np.zeros(2, dtype=np.int32)
         _lib.check(_lib.load().lcc_kv4_prefill_plan(new.ctypes.data, past.ctypes.data, len(seg), int(n_q_heads), int(n_kv_heads), cus, plan[0:].ctypes.data,
                                                     plan[1:].ctypes.data), "lcc_kv4_prefill_plan")
-        self.tile_rows, self.nsplit = int(plan[0]), int(nsplit) if nsplit > 0 else int(plan[1])
+        self.tile_rows, self.nsplit = int(tile_rows) if tile_rows > 0 else int(plan[0]), int(nsplit) if nsplit > 0 else int(plan[1])
         self.n_q_heads, self.n_kv_heads, self.rows = int(n_q_heads), int(n_kv_heads), int(new.sum())
         self.max_keys = int((new.astype(np.int64) + past)[new > 0].max(initial=0))
         tiles, row = [], 0
@@ -590,9 +590,10 @@ class Kv4PrefillPlan:
         self.tiles = torch.as_tensor(np.ascontiguousarray(np.asarray(tiles, dtype=np.int32).reshape(-1, 4).T), device=device)
 
 
-def kv4_prefill_plan(segments: Sequence[Tuple[int, int, int]], n_q_heads: int, n_kv_heads: int, device, nsplit: int = 0) -> Kv4PrefillPlan:
-    """segments: (slot, n_new, past_len) per stream, rows packed in that order.  nsplit 0: the split count that suits them (lcc_kv4_prefill_plan)."""
-    return Kv4PrefillPlan(segments, n_q_heads, n_kv_heads, device, nsplit)
+def kv4_prefill_plan(segments: Sequence[Tuple[int, int, int]], n_q_heads: int, n_kv_heads: int, device, nsplit: int = 0, tile_rows: int = 0) -> Kv4PrefillPlan:
+    """segments: (slot, n_new, past_len) per stream, rows packed in that order.  nsplit, tile_rows 0: the split count and tile height that suit them
+    (lcc_kv4_prefill_plan)."""
+    return Kv4PrefillPlan(segments, n_q_heads, n_kv_heads, device, nsplit, tile_rows)
 
 
 def attn_prefill4(q: torch.Tensor, kv: Kv4Arena, layer: int, plan, n_q_heads: int) -> torch.Tensor:

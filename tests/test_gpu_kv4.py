@@ -307,13 +307,15 @@ def test_decode_nan_reaches_the_channels_and_heads_that_read_it(dev):
 @pytest.mark.parametrize("heads,kv_heads", [(2, 1), (7, 1), (28, 4), (3, 3), (32, 2), (64, 8)])
 @pytest.mark.parametrize("segments", [[(0, 1, 0)], [(1, 5, 59)], [(0, 37, 0), (1, 3, 61), (2, 0, 5), (0, 2, 37)], [(2, 33, 30), (1, 64, 32)]])
 @pytest.mark.parametrize("nsplit", [1, 3])
-def test_chunk(dev, heads, kv_heads, segments, nsplit):
+@pytest.mark.parametrize("columns", [16, 128, 256])
+def test_chunk(dev, heads, kv_heads, segments, nsplit, columns):
+    """the three kernels: tiles of up to 16, 128 and 256 (row, head) columns"""
     from livecc_amd import ops
     L = 96
     kv = filled(dev, rand((3, kv_heads, L, 128), dev, 1), rand((3, kv_heads, L, 128), dev, 2))
     S = sum(n for _, n, _ in segments)
     q = rand((S, heads * 128), dev, 3)
-    plan = ops.kv4_prefill_plan(segments, heads, kv_heads, dev, nsplit)
+    plan = ops.kv4_prefill_plan(segments, heads, kv_heads, dev, nsplit, columns * kv_heads // heads)
     got = ops.attn_prefill4(q, kv, 0, plan, heads)
     row = 0
     for slot, n, past in segments:
@@ -327,14 +329,15 @@ def test_chunk(dev, heads, kv_heads, segments, nsplit):
         U.assert_within(ops.attn_prefill4(q, kv, 0, segments, heads)[row - n:row], want.flatten(1), tol.flatten(1))
 
 
-@pytest.mark.parametrize("rows,past,heads,kv_heads", [(150, 1000, 7, 1), (2, 700, 28, 4), (300, 0, 12, 2)])
-def test_chunk_longer(dev, rows, past, heads, kv_heads):
+@pytest.mark.parametrize("rows,past,heads,kv_heads", [(150, 1000, 7, 1), (2, 700, 28, 4), (300, 0, 12, 2), (20, 5000, 28, 4)])
+@pytest.mark.parametrize("columns", [0, 16, 128, 256])
+def test_chunk_longer(dev, rows, past, heads, kv_heads, columns):
     from livecc_amd import ops
     L = rows + past
     kv = filled(dev, rand((1, kv_heads, L, 128), dev, 1, 2.0), rand((1, kv_heads, L, 128), dev, 2))
     q = rand((rows, heads * 128), dev, 3, 1.5)
     kk, vv = values(kv, 0)
-    got = ops.attn_prefill4(q, kv, 0, [(0, rows, past)], heads)
+    got = ops.attn_prefill4(q, kv, 0, ops.kv4_prefill_plan([(0, rows, past)], heads, kv_heads, dev, 0, columns * kv_heads // heads), heads)
     at = sorted({0, 1, rows // 2, rows - 2, rows - 1} & set(range(rows)))
     want, tol = U.attention(q[at].cpu().view(len(at), heads, 128), kk, vv, [past + r for r in at])
     U.assert_within(got[at], want.flatten(1), tol.flatten(1))
@@ -345,7 +348,8 @@ def test_chunk_longer(dev, rows, past, heads, kv_heads):
     assert bool((wide <= 2.0 ** -7 * top + 2.0 ** -7 * one.float().abs()).all())
 
 
-def test_chunk_rows_do_not_see_later_keys(dev):
+@pytest.mark.parametrize("columns", [16, 128, 256])
+def test_chunk_rows_do_not_see_later_keys(dev, columns):
     """NaN keys and values of later rows of the same chunk, and garbage behind the stream's last key, reach no earlier row; the rows that see them are NaN where they are."""
     from livecc_amd import ops
     heads, kv_heads, L, past, n = 14, 2, 128, 50, 40
@@ -366,16 +370,17 @@ def test_chunk_rows_do_not_see_later_keys(dev):
     want[16:, 7:, 96:] = math.nan
     want[30:, 7:] = math.nan
     for nsplit in (1, 2):
-        got = ops.attn_prefill4(q, kv, 0, ops.kv4_prefill_plan([(0, n, past)], heads, kv_heads, dev, nsplit), heads)
+        got = ops.attn_prefill4(q, kv, 0, ops.kv4_prefill_plan([(0, n, past)], heads, kv_heads, dev, nsplit, columns * kv_heads // heads), heads)
         U.assert_within(got, want.flatten(1), tol.flatten(1), f"nsplit {nsplit}")
 
 
-def test_chunk_of_a_slot_that_does_not_exist(dev):
+@pytest.mark.parametrize("columns", [16, 128, 256])
+def test_chunk_of_a_slot_that_does_not_exist(dev, columns):
     from livecc_amd import ops
     kv = filled(dev, rand((2, 1, 64, 128), dev, 1), rand((2, 1, 64, 128), dev, 2))
     q = rand((9, 7 * 128), dev, 3)
     for nsplit in (1, 2):
-        got = ops.attn_prefill4(q, kv, 0, ops.kv4_prefill_plan([(-1, 3, 0), (1, 3, 20), (2, 3, 4)], 7, 1, dev, nsplit), 7)
+        got = ops.attn_prefill4(q, kv, 0, ops.kv4_prefill_plan([(-1, 3, 0), (1, 3, 20), (2, 3, 4)], 7, 1, dev, nsplit, columns // 7), 7)
         assert not got[:3].any() and not got[6:].any() and bool(got[3:6].any())
 
 
@@ -532,7 +537,8 @@ def test_refusals(dev, through, monkeypatch):
                 lambda: ops.attn_prefill4(qkv[:, :512].contiguous(), kv, 0, [(0, 2, 0)], heads),
                 lambda: ops.attn_prefill4(qkv[:, :512].contiguous(), kv, 0, [(0, 3, 62)], heads),
                 lambda: ops.attn_prefill4(qkv[:, :512].contiguous(), kv, 0, ops.kv4_prefill_plan([(0, 3, 0)], heads, kv_heads, dev, 65), heads),
-                lambda: ops.attn_prefill4(qkv[:, :512].contiguous(), kv, 0, ops.kv4_prefill_plan([(0, 3, 0)], 8, kv_heads, dev), heads)):
+                lambda: ops.attn_prefill4(qkv[:, :512].contiguous(), kv, 0, ops.kv4_prefill_plan([(0, 3, 0)], 8, kv_heads, dev), heads),
+                lambda: ops.attn_prefill4(qkv[:, :512].contiguous(), kv, 0, ops.kv4_prefill_plan([(0, 3, 0)], heads, kv_heads, dev, 0, 129), heads)):
         with pytest.raises(err):
             bad()
     assert not kv.buf.any()
