@@ -925,10 +925,11 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_chunk_kv4_kernel(Kv4Args a, c
 
 // Tile height -- which of the three kernels -- and key splits, by a cost in us.  All: 4 for the launch and the way to the first key; splits another launch (3) and their
 // partials, 1,040 bytes a row, head and split written and read at 4.5 TB/s.
-//   16 columns (attn_rows_kv4_kernel): a wave's 32-key block takes 1.1 when waves are few and 0.75 of a SIMD's time when they are many.
-//   128 or 256 columns (attn_chunk_kv4_kernel of four waves, two blocks a unit, or eight): a stage of 64 keys 1.6 (four waves: alone on a unit 1.2, two blocks 1.8), a block's prologue
-//   and result as 2.5 stages; blocks
-//   that all run at once take as long as the longest, more of them the mean and most of one.
+//   16 columns (attn_rows_kv4_kernel): a wave's 32-key block takes 1.1 when waves are few and 0.75 of a SIMD's time when they are many, a block of eight waves 1.7
+//   besides.
+//   128 or 256 columns (attn_chunk_kv4_kernel of four waves, two blocks a unit, or eight): a stage of 64 keys 1.6 (four waves: alone on a unit 1.2, two blocks 1.8), 3
+//   stages for a block's prologue and result and 3 for the masked end; blocks that all run at once take as long as the longest, more of them (longest first) the mean
+//   and half of one.
 // Measured, 16 / 128 columns (us): 28 / 4 heads on 26,000 keys 2 rows 11.8 / 20.3, 8 rows 17.3 / 23.5, 12 rows 22.5 / 25.3, 18 rows 29.6 / 27.2; 18 rows on 500 keys of
 // 64 / 8 heads 7.9 / 15.8; 8 x 18 rows on 3,000 keys 30.3 / 27.7.  128 / 256 columns: 8 x ~340 rows on ~5,000 keys 266 / 263, 386 rows on 6,100 60 / 56.
 int kv4_prefill_plan(const int32_t* n_new, const int32_t* past, int n, int n_q_heads, int n_kv_heads, int cus, int* tile_rows, int* nsplit) {
@@ -960,10 +961,11 @@ int kv4_prefill_plan(const int32_t* n_new, const int32_t* past, int n, int n_q_h
       float cost = 4.f + (k > 1 ? 3.f + join * k : 0.f);
       if (columns == 16) {
         const float one = 1.1f * (float)((longest + (k == 1 ? 8 : 4) * k - 1) / ((k == 1 ? 8 : 4) * k)), all = work * 0.75f / (4.f * cus);
-        cost += std::max(one, all + (blocks > cus ? 0.5f * one : 0.f));
+        cost += std::max(one, all + (blocks > cus ? 0.5f * one + (k == 1 ? 1.7f : 0.85f) * (blocks / cus - 1.f) : 0.f));
       } else {
-        const float slots = (float)cus * (columns == 128 ? 2 : 1), block = (float)longest / k + 2.5f;
-        cost += blocks <= slots ? (columns == 256 ? 1.6f : blocks <= cus ? 1.2f : 1.8f) * block : 1.6f * ((work + 2.5f * blocks) / slots * (columns == 128 ? 1.5f : 1.f) + 0.8f * block);
+        const float slots = (float)cus * (columns == 128 ? 2 : 1), block = (float)longest / k + 6.f;
+        cost += blocks <= slots ? (columns == 256 ? 1.6f : blocks <= cus ? 1.2f : 1.8f) * block
+                                : (columns == 256 ? 1.6f : 1.5f) * ((work + 3.f * blocks + 3.f * tiles * n_kv_heads) / slots + 0.5f * block);
       }
       if (cost < best) { best = cost; *tile_rows = height; *nsplit = k; }
     }

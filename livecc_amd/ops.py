@@ -587,6 +587,7 @@ class Kv4PrefillPlan:
         for slot, n, p in seg.tolist():
             tiles += [(slot, row + o, min(self.tile_rows, n - o), p + o) for o in range(0, n, self.tile_rows)]
             row += n
+        tiles.sort(key=lambda t: -(t[2] + t[3]))          # the longest first: blocks start in this order
         self.tiles = torch.as_tensor(np.ascontiguousarray(np.asarray(tiles, dtype=np.int32).reshape(-1, 4).T), device=device)
 
 
