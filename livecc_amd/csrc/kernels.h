@@ -387,7 +387,9 @@ struct Kv4Layout {  // a slot's layer: [K codes | V codes | K scales | V scales]
 };
 struct Kv4Args {
   void* const* kv_base; int n_slots, n_layers, n_kv_heads, lmax, layer;
-  int check() const { return n_slots < 0 || n_layers < 1 || n_kv_heads < 1 || lmax < 32 || (lmax & 31) || layer < 0 || layer >= n_layers ? LCC_ERR_SHAPE : 0; }
+  int check() const {
+    return n_slots < 0 || n_layers < 1 || n_kv_heads < 1 || n_kv_heads > 65535 || lmax < 32 || lmax > 1 << 30 || (lmax & 31) || layer < 0 || layer >= n_layers ? LCC_ERR_SHAPE : 0;
+  }
 };
 struct QkNormArgs {
   const bf16_t* qkv; const float* partial; int nsplit; const bf16_t* bias;      // rows [q heads | k heads | v heads][128]: bf16, or slabs (+ bias)

@@ -362,8 +362,8 @@ __global__ __launch_bounds__(256) void qk_norm_rope_append_kernel(QkNormArgs a, 
 }
 
 static int qk_norm_check(const QkNormArgs& a) {
-  if (a.rows < 0 || a.n_q_heads < 0 || a.n_kv_heads < 1 || a.lmax < 32 || (a.lmax & 31) || a.n_layers < 1 || a.layer < 0 || a.layer >= a.n_layers || a.n_slots < 0)
-    return LCC_ERR_SHAPE;
+  if (int rc = Kv4Args{a.kv_base, a.n_slots, a.n_layers, a.n_kv_heads, a.lmax, a.layer}.check()) return rc;
+  if (a.rows < 0 || a.n_q_heads < 0 || a.n_q_heads > 65535) return LCC_ERR_SHAPE;
   if (a.partial != nullptr && (a.nsplit < 1 || a.nsplit > 8)) return LCC_ERR_SHAPE;
   if (!(a.eps > 0.f) && (a.q_norm != nullptr || a.k_norm != nullptr)) return LCC_ERR_ARG;
   return 0;
@@ -663,8 +663,8 @@ static void attn_rows_launch(const Kv4Args& a, const Kv4Rows& rows, int n, const
 int attn_decode_kv4(const Kv4Args& a, const bf16_t* q, const int32_t* slots, const int32_t* kv_len, int rows, int n_q_heads, int nsplit, float* ws_o, float* ws_ml,
                     bf16_t* out, hipStream_t st) {
   if (int rc = a.check()) return rc;
-  if (rows < 0 || rows > 65535 || n_q_heads < 1 || n_q_heads % a.n_kv_heads || n_q_heads / a.n_kv_heads > 16 || nsplit < 1 || nsplit > 64 || a.n_kv_heads > 65535)
-    return LCC_ERR_SHAPE;
+  if (rows < 0 || rows > 65535 || n_q_heads < 1 || n_q_heads % a.n_kv_heads || n_q_heads / a.n_kv_heads > 16 || nsplit < 1 || nsplit > 64) return LCC_ERR_SHAPE;
+  if ((int64_t)rows * n_q_heads > 0x7fffffff) return LCC_ERR_SHAPE;
   if (nsplit > 1 && (ws_o == nullptr || ws_ml == nullptr)) return LCC_ERR_ARG;
   if (rows == 0) return 0;
   attn_rows_launch<false>(a, Kv4Rows{slots, kv_len, nullptr, nullptr, nullptr, 1, rows}, rows, q, n_q_heads, nsplit, ws_o, ws_ml, out, st);
@@ -978,7 +978,7 @@ int attn_prefill_kv4(const Kv4Args& a, const bf16_t* q, bf16_t* out, const int32
   if (int rc = a.check()) return rc;
   if (n_tiles < 0 || n_tiles > 65535 || n_rows < 0 || n_q_heads < 1 || n_q_heads % a.n_kv_heads || n_q_heads / a.n_kv_heads > 16 || nsplit < 1 || nsplit > 64)
     return LCC_ERR_SHAPE;
-  if (tile_rows < 1 || tile_rows > 256 / (n_q_heads / a.n_kv_heads)) return LCC_ERR_SHAPE;
+  if (tile_rows < 1 || tile_rows > 256 / (n_q_heads / a.n_kv_heads) || (int64_t)n_rows * n_q_heads > 0x7fffffff) return LCC_ERR_SHAPE;
   if (nsplit > 1 && (ws_o == nullptr || ws_ml == nullptr)) return LCC_ERR_ARG;
   if (n_tiles == 0 || n_rows == 0) return 0;
   static DeviceOnce once;

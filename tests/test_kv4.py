@@ -127,7 +127,7 @@ def test_c_entries_refuse_before_any_launch(built_lib):
         for kw in (dict(qkv=odd), dict(qn=odd), dict(kn=odd), dict(cos=odd), dict(sin=odd), dict(q=odd)):
             assert append(fn, **kw) == ERR_ALIGN, kw
         for kw in (dict(lay=_lib.KvLayout(1, 2, 64, 64)), dict(lay=_lib.KvLayout(1, 2, 48, 128)), dict(lay=_lib.KvLayout(1, 0, 64, 128)), dict(layer=1), dict(layer=-1), dict(S=-1),
-                   dict(H=-1), dict(slots=-1), dict(qkv=None, part=p, nsplit=0), dict(qkv=None, part=p, nsplit=9)):
+                   dict(H=-1), dict(H=65536), dict(slots=-1), dict(lay=_lib.KvLayout(1, 2, (1 << 30) + 32, 128)), dict(S=0x7fffffff), dict(qkv=None, part=p, nsplit=0), dict(qkv=None, part=p, nsplit=9)):
             assert append(fn, **kw) == ERR_SHAPE, kw
 
     def read(**kw):
@@ -143,7 +143,7 @@ def test_c_entries_refuse_before_any_launch(built_lib):
         return lib.lcc_attn_decode_kv4(*a.values(), None)
     assert [decode(**{n: None}) for n in ("q", "out", "slots", "length", "base")] == [ERR_ARG] * 5
     assert decode(nsplit=2) == decode(nsplit=2, o=p) == ERR_ARG
-    for kw in (dict(H=3), dict(H=34), dict(H=0), dict(nsplit=0), dict(nsplit=65, o=p, ml=p), dict(B=-1), dict(B=65536), dict(layer=1), dict(lay=_lib.KvLayout(1, 2, 33, 128))):
+    for kw in (dict(H=3), dict(H=34), dict(H=0), dict(nsplit=0), dict(nsplit=65, o=p, ml=p), dict(B=-1), dict(B=65536), dict(B=65535, H=65536, lay=_lib.KvLayout(1, 8192, 32, 128)), dict(layer=1), dict(lay=_lib.KvLayout(1, 2, 33, 128))):
         assert decode(**kw) == ERR_SHAPE, kw
     assert decode(q=odd) == decode(out=odd) == decode(o=odd, ml=p, nsplit=2) == ERR_ALIGN
 
@@ -153,7 +153,7 @@ def test_c_entries_refuse_before_any_launch(built_lib):
         return lib.lcc_attn_prefill_kv4(*a.values(), None)
     assert [chunk(**{n: None}) for n in ("q", "out", "t0", "t1", "t2", "t3", "base")] == [ERR_ARG] * 7
     assert chunk(nsplit=2) == ERR_ARG
-    for kw in (dict(H=3), dict(H=34), dict(nsplit=0), dict(nsplit=65, o=p, ml=p), dict(tiles=-1), dict(tiles=65536), dict(rows=0), dict(rows=129), dict(S=-1), dict(layer=1)):
+    for kw in (dict(H=3), dict(H=34), dict(nsplit=0), dict(nsplit=65, o=p, ml=p), dict(tiles=-1), dict(tiles=65536), dict(rows=0), dict(rows=129), dict(S=-1), dict(S=1 << 30), dict(layer=1)):
         assert chunk(**kw) == ERR_SHAPE, kw
     assert chunk(q=odd) == chunk(out=odd) == ERR_ALIGN
 
