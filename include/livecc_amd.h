@@ -346,7 +346,7 @@ int lcc_kv4_decode_splits(const int32_t* n_keys, int n_streams, int n_kv_heads);
 int lcc_attn_decode_kv4(const void* q, void* out, const int32_t* slots, const int32_t* kv_len, void* const* kv_base, int n_slots, lcc_kv_layout lay, int layer, int B,
                         int n_q_heads, int nsplit, float* ws_o, float* ws_ml, void* stream);
 /* attention core as lcc_attn_prefill_bf16 over the 4-bit cache: tiles of up to tile_rows (<= 256 / (Hq / Hkv)) consecutive new rows of one stream; a row at
- * position p sees keys 0 .. p.  Every row of q belongs to exactly one tile.  nsplit <= 64; > 1: scratch ws_o [n_rows * Hq * nsplit * 128], ws_ml [n_rows * Hq *
+ * position p sees keys 0 .. p.  A row of q belongs to at most one tile; rows of none are left as they are in out.  nsplit <= 64; > 1: scratch ws_o [n_rows * Hq * nsplit * 128], ws_ml [n_rows * Hq *
  * nsplit * 2].  lcc_kv4_prefill_plan: tile height and split count for streams of n_new[b] rows behind past[b] keys on a device of cu_count compute units (host logic) */
 int lcc_kv4_prefill_plan(const int32_t* n_new, const int32_t* past, int n_streams, int n_q_heads, int n_kv_heads, int cu_count, int32_t* tile_rows, int32_t* nsplit);
 int lcc_attn_prefill_kv4(const void* q, void* out, const int32_t* tile_stream, const int32_t* tile_q0, const int32_t* tile_nq, const int32_t* tile_pos0,

@@ -385,10 +385,12 @@ struct Kv4Layout {  // a slot's layer: [K codes | V codes | K scales | V scales]
   __host__ __device__ size_t k_scales(int h) const { return (size_t)n_kv_heads * lmax * 128 + (size_t)h * lmax * 4; }
   __host__ __device__ size_t v_scales(int h) const { return (size_t)n_kv_heads * lmax * 132 + (size_t)h * lmax * 4; }
 };
+constexpr int KV4_MAX_LMAX = 1 << 30, KV4_MAX_PLANES = 1 << 24;    // keys of a head, heads * layers: every offset in a slot fits 63 bits
 struct Kv4Args {
   void* const* kv_base; int n_slots, n_layers, n_kv_heads, lmax, layer;
   int check() const {
-    return n_slots < 0 || n_layers < 1 || n_kv_heads < 1 || n_kv_heads > 65535 || lmax < 32 || lmax > 1 << 30 || (lmax & 31) || layer < 0 || layer >= n_layers ? LCC_ERR_SHAPE : 0;
+    return n_slots < 0 || n_layers < 1 || n_kv_heads < 1 || n_kv_heads > 65535 || (int64_t)n_layers * n_kv_heads > KV4_MAX_PLANES || lmax < 32 || lmax > KV4_MAX_LMAX ||
+           (lmax & 31) || layer < 0 || layer >= n_layers ? LCC_ERR_SHAPE : 0;
   }
 };
 struct QkNormArgs {

@@ -59,20 +59,6 @@ template <int SEL>
 LCC_DEVICE unsigned scale_of(unsigned w) { return SEL < 3 ? w << (23 - 8 * SEL) : w >> 1; }
 // a word of K codes -> eight channels
 LCC_DEVICE u32x4 fp4_word(unsigned w, unsigned scale) { return (u32x4){fp4_pair<0>(w, scale), fp4_pair<1>(w, scale), fp4_pair<2>(w, scale), fp4_pair<3>(w, scale)}; }
-// eight V bytes (keys 0..7 of an octet) and their eight scale bytes -> the octet's values of channel i (lo) and i + 16 (hi)
-LCC_DEVICE void fp4_octet(u32x2 w, u32x2 s, u32x4& lo, u32x4& hi) {
-  unsigned c[8];
-#pragma unroll
-  for (int d = 0; d < 2; ++d) {
-    c[4 * d] = fp4_pair<0>(w[d], scale_of<0>(s[d])); c[4 * d + 1] = fp4_pair<1>(w[d], scale_of<1>(s[d]));
-    c[4 * d + 2] = fp4_pair<2>(w[d], scale_of<2>(s[d])); c[4 * d + 3] = fp4_pair<3>(w[d], scale_of<3>(s[d]));
-  }
-#pragma unroll
-  for (int d = 0; d < 4; ++d) {
-    lo[d] = __builtin_amdgcn_perm(c[2 * d + 1], c[2 * d], 0x05040100u);
-    hi[d] = __builtin_amdgcn_perm(c[2 * d + 1], c[2 * d], 0x07060302u);
-  }
-}
 
 // ------------------------------------------------------------------------------------------------------------------------------
 // Norm, rotation, append.
@@ -374,7 +360,7 @@ int qk_norm_rope_append(const QkNormArgs& a, bool kv4, hipStream_t st) {
   const bool windows = a.rows >= KV4_WINDOW_ROWS;
   const int64_t items = (int64_t)a.rows * (a.n_q_heads + (windows ? 1 : 2) * a.n_kv_heads), blocks = (items + 31) / 32;
   const int64_t v_blocks = windows ? ((int64_t)a.rows + 31) / 32 * a.n_kv_heads : 0;
-  if (items > 0x7fffff00 || blocks + v_blocks > 0x7fffffff) return LCC_ERR_SHAPE;
+  if (blocks + v_blocks >= 1 << 24) return LCC_ERR_SHAPE;                    // a launch has fewer than 2^32 threads
   const dim3 grid((unsigned)(blocks + v_blocks));
   const int every = windows ? (int)(((blocks + v_blocks) / v_blocks - 1) | 1) : 1;         // V blocks among the others, an odd number apart: blocks go round the eight XCDs
   if (windows && kv4) qk_norm_rope_append_kernel<true, true><<<grid, dim3(256), 0, st>>>(a, (int)v_blocks, every);
@@ -419,7 +405,7 @@ int kv4_read(const Kv4Args& a, const int32_t* tok_stream, const int32_t* tok_pos
   if (rows < 0) return LCC_ERR_SHAPE;
   if (rows == 0) return 0;
   const int64_t blocks = ((int64_t)rows * a.n_kv_heads + 31) / 32;
-  if (blocks > 0x7fffffff) return LCC_ERR_SHAPE;
+  if (blocks >= 1 << 24) return LCC_ERR_SHAPE;
   kv4_read_kernel<<<dim3((unsigned)blocks), dim3(256), 0, st>>>(a, tok_stream, tok_pos, k, v, rows);
   return 0;
 }
@@ -537,7 +523,7 @@ __global__ __launch_bounds__(NW * 64, 4) void attn_rows_kv4_kernel(Kv4Args a, Kv
         for (int t = 0; t < 8; ++t) o[t] *= f;
         m = mn;
       }
-      const float mu = CHUNK && m == -INFINITY ? 0.f : m;                   // a column that has seen no key
+      const float mu = m == -INFINITY ? 0.f : m;                            // a column that has seen no key, or scores of -inf alone
       float p[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) { p[e] = __builtin_amdgcn_exp2f(fmaf(sc[e >> 2][e & 3], scale_log2e, -mu)); l += p[e]; }
@@ -595,14 +581,18 @@ __global__ __launch_bounds__(NW * 64, 4) void attn_rows_kv4_kernel(Kv4Args a, Kv
 }
 
 // Joins the key splits of a (row, head): sums weighted by 2^(m - max), one rounding.  A half-wave reads a split's 128 channels at a time; W waves share a (row, head).
+// blockIdx.y: a tile, or (tiles null) a row.
 template <int W>
-__global__ __launch_bounds__(256) void kv4_combine_kernel(const float* __restrict__ ws_o, const float* __restrict__ ws_ml, bf16_t* __restrict__ out, int64_t n, int nsplit) {
+__global__ __launch_bounds__(256) void kv4_combine_kernel(const float* __restrict__ ws_o, const float* __restrict__ ws_ml, bf16_t* __restrict__ out,
+                                                          const int32_t* __restrict__ tile_q0, const int32_t* __restrict__ tile_nq, int tile_rows, int n_rows, int n_q_heads,
+                                                          int nsplit) {
   __shared__ f32x4 so[W][32];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, c = lane & 31;
-  const int64_t row = W == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
-  if (row >= n) return;                                                     // whole waves, and W > 1: none
-  const float* ml = ws_ml + (size_t)row * nsplit * 2;
-  const float* o = ws_o + (size_t)row * nsplit * 128 + c * 4;
+  const int item = W == 1 ? blockIdx.x * 4 + wave : blockIdx.x, b = blockIdx.y, q0 = tile_q0 ? tile_q0[b] : b;
+  if (q0 < 0 || item >= min(tile_q0 ? min(tile_nq[b], tile_rows) : 1, n_rows - q0) * n_q_heads) return;       // whole waves; W > 1: whole blocks
+  const size_t row = (size_t)q0 * n_q_heads + item;
+  const float* ml = ws_ml + row * nsplit * 2;
+  const float* o = ws_o + row * nsplit * 128 + c * 4;
   constexpr int N = W == 1 ? 4 : 8;                                          // a half-wave's share of 8 or 64 splits, all in flight before the weights are formed
   const int s0 = wave * (W == 1 ? 0 : 2) + half;
   f32x4 v[N];
@@ -632,11 +622,13 @@ __global__ __launch_bounds__(256) void kv4_combine_kernel(const float* __restric
     for (int i = 1; i < W; ++i) acc += so[i][c];
   }
   const float r = L == 0.f ? 0.f : 1.f / L;
-  if (half == 0) st8(out + (size_t)row * 128 + c * 4, (u32x2){pack2(acc[0] * r, acc[1] * r), pack2(acc[2] * r, acc[3] * r)});
+  if (half == 0) st8(out + row * 128 + c * 4, (u32x2){pack2(acc[0] * r, acc[1] * r), pack2(acc[2] * r, acc[3] * r)});
 }
-static void kv4_combine(const float* ws_o, const float* ws_ml, bf16_t* out, int64_t n, int nsplit, hipStream_t st) {
-  if (nsplit <= 8) kv4_combine_kernel<1><<<dim3((unsigned)((n + 3) / 4)), dim3(256), 0, st>>>(ws_o, ws_ml, out, n, nsplit);
-  else kv4_combine_kernel<4><<<dim3((unsigned)n), dim3(256), 0, st>>>(ws_o, ws_ml, out, n, nsplit);
+static void kv4_combine(const float* ws_o, const float* ws_ml, bf16_t* out, const int32_t* tile_q0, const int32_t* tile_nq, int n_tiles, int tile_rows, int n_rows,
+                        int n_q_heads, int nsplit, hipStream_t st) {
+  const unsigned items = (unsigned)tile_rows * n_q_heads;                   // up to 256 * 65535
+  if (nsplit <= 8) kv4_combine_kernel<1><<<dim3((items + 3) / 4, n_tiles), dim3(256), 0, st>>>(ws_o, ws_ml, out, tile_q0, tile_nq, tile_rows, n_rows, n_q_heads, nsplit);
+  else kv4_combine_kernel<4><<<dim3(items, n_tiles), dim3(256), 0, st>>>(ws_o, ws_ml, out, tile_q0, tile_nq, tile_rows, n_rows, n_q_heads, nsplit);
 }
 
 int kv4_decode_splits(const int32_t* n_keys, int n, int n_kv_heads) {
@@ -668,7 +660,7 @@ int attn_decode_kv4(const Kv4Args& a, const bf16_t* q, const int32_t* slots, con
   if (nsplit > 1 && (ws_o == nullptr || ws_ml == nullptr)) return LCC_ERR_ARG;
   if (rows == 0) return 0;
   attn_rows_launch<false>(a, Kv4Rows{slots, kv_len, nullptr, nullptr, nullptr, 1, rows}, rows, q, n_q_heads, nsplit, ws_o, ws_ml, out, st);
-  if (nsplit > 1) kv4_combine(ws_o, ws_ml, out, (int64_t)rows * n_q_heads, nsplit, st);
+  if (nsplit > 1) kv4_combine(ws_o, ws_ml, out, nullptr, nullptr, rows, 1, rows, n_q_heads, nsplit, st);
   return 0;
 }
 
@@ -994,7 +986,7 @@ int attn_prefill_kv4(const Kv4Args& a, const bf16_t* q, bf16_t* out, const int32
     attn_chunk_kv4_kernel<8><<<grid, dim3(512), KV4_LDS, st>>>(a, q, out, tile_stream, tile_q0, tile_nq, tile_pos0, n_q_heads, tile_rows, nsplit, n_rows, ws_o, ws_ml, scale);
   else
     attn_chunk_kv4_kernel<4><<<grid, dim3(256), KV4_LDS, st>>>(a, q, out, tile_stream, tile_q0, tile_nq, tile_pos0, n_q_heads, tile_rows, nsplit, n_rows, ws_o, ws_ml, scale);
-  if (nsplit > 1) kv4_combine(ws_o, ws_ml, out, (int64_t)n_rows * n_q_heads, nsplit, st);
+  if (nsplit > 1) kv4_combine(ws_o, ws_ml, out, tile_q0, tile_nq, n_tiles, tile_rows, n_rows, n_q_heads, nsplit, st);
   return 0;
 }
 

@@ -536,8 +536,8 @@ extern "C" int lcc_latent_attn_decode(const void* q_latent, const int32_t* slots
 static Kv4Args to_kv4(void* const* kv_base, int n_slots, lcc_kv_layout lay, int layer) { return Kv4Args{kv_base, n_slots, lay.n_layers, lay.n_kv_heads, lay.lmax, layer}; }
 static int kv4_lay_ok(lcc_kv_layout lay, const char* name) {
   if (lay.head_dim != 128) return fail(LCC_ERR_SHAPE, "%s: head_dim must be 128, got %d", name, lay.head_dim);
-  if (lay.n_layers < 1 || lay.n_kv_heads < 1 || lay.n_kv_heads > 65535 || lay.lmax < 32 || lay.lmax > 1 << 30 || lay.lmax % 32)
-    return fail(LCC_ERR_SHAPE, "%s: bad cache layout (lmax a multiple of 32, up to 2^30)", name);
+  if (Kv4Args{nullptr, 0, lay.n_layers, lay.n_kv_heads, lay.lmax, 0}.check())
+    return fail(LCC_ERR_SHAPE, "%s: bad cache layout (lmax a multiple of 32, up to 2^30; up to 65535 heads, 2^24 heads of all layers)", name);
   return 0;
 }
 static bool not16(const void* p) { return ((uintptr_t)p & 15) != 0; }

@@ -225,7 +225,7 @@ Cache cache_of(const Tensor& like, const Tensor& kv_ptrs, const Tensor& kv_buf, 
               "kv_buf: contiguous uint8", bf16_too ? " or bf16" : "", " GPU tensor [n_slots, slot] expected");
   TORCH_CHECK(kv_ptrs.device() == like.device() && kv_buf.device() == like.device(), "the cache must be on the device of the rows");
   TORCH_CHECK(kv_ptrs.numel() == kv_buf.size(0), "kv_ptrs: one entry per slot expected");
-  TORCH_CHECK(n_layers >= 1 && n_layers <= 65535 && n_kv_heads >= 1 && n_kv_heads <= 65535 && lmax >= 32 && lmax <= 1 << 30 && (lmax % 32) == 0 && layer >= 0 && layer < n_layers,
+  TORCH_CHECK(n_layers >= 1 && n_layers <= 1 << 24 && n_kv_heads >= 1 && n_kv_heads <= 65535 && n_layers * n_kv_heads <= 1 << 24 && lmax >= 32 && lmax <= 1 << 30 && (lmax % 32) == 0 && layer >= 0 && layer < n_layers,
               "bad cache layout / layer");
   const lcc_kv_layout lay = layout_of(n_layers, n_kv_heads, lmax);
   const int64_t need = kv4 ? (int64_t)lcc_kv4_slot_bytes(lay) : n_layers * 2 * n_kv_heads * lmax * 128;

@@ -570,3 +570,51 @@ def test_through_the_c_abi_as_through_torch(dev, bits, monkeypatch):
     monkeypatch.setattr(torch_ops, "op", lambda name: None)
     for x, y in zip(a, go()):
         assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("columns", [16, 128, 256])
+@pytest.mark.parametrize("nsplit", [1, 3, 12])
+def test_chunk_rows_of_no_tile_stay_as_they_were(dev, columns, nsplit):
+    """Rows between and behind the tiles, whatever the workspace holds for them; a tile that says more rows than q has."""
+    import ctypes
+    from livecc_amd import _lib, ops
+    heads, kv_heads, L = 14, 2, 96
+    kv = filled(dev, rand((2, kv_heads, L, 128), dev, 1), rand((2, kv_heads, L, 128), dev, 2))
+    S, height = 40, columns * kv_heads // heads
+    tiles = [(0, 2, min(2, height), 50), (1, 10, min(9, height), 80), (0, 38, height, 0)]
+    q, out = rand((S, heads * 128), dev, 3), rand((S, heads * 128), dev, 4)
+    before, t = out.clone(), i32([list(c) for c in zip(*tiles)], dev)
+    ws = torch.full((S * heads * nsplit * 130,), math.nan, device=dev)
+    at, st = t.data_ptr(), ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    _lib.check(_lib.load().lcc_attn_prefill_kv4(q.data_ptr(), out.data_ptr(), at, at + 12, at + 24, at + 36, kv.ptrs.data_ptr(), 2, kv.lay, 0, 3, heads, height, nsplit, S,
+                                                ws.data_ptr(), ws.data_ptr() + S * heads * nsplit * 512, st), "lcc_attn_prefill_kv4")
+    left = set(range(S))
+    for slot, q0, nq, pos in tiles:
+        nq = min(nq, S - q0)
+        want, tol = U.attention(q[q0:q0 + nq].cpu().view(nq, heads, 128), *values(kv, slot), [pos + r for r in range(nq)])
+        U.assert_within(out[q0:q0 + nq], want.flatten(1), tol.flatten(1), f"rows {q0}..")
+        left -= set(range(q0, q0 + nq))
+    left = sorted(left)
+    assert torch.equal(out[left], before[left])
+
+
+@pytest.mark.parametrize("columns", [0, 16, 128, 256])
+@pytest.mark.parametrize("nsplit", [1, 2])
+def test_keys_whose_scores_are_minus_infinity(dev, columns, nsplit):
+    """The first 64 keys' scores leave the type's range downwards, the others' are zero: the mean of the others' values.  Tolerance: half a step of bf16 for the
+    result, none for the probabilities (all one), 2^-16 for the sums.  columns 0: single tokens."""
+    from livecc_amd import ops
+    heads, kv_heads, L = 14, 2, 320
+    k, v = torch.zeros(1, kv_heads, L, 128, dtype=torch.bfloat16, device=dev), rand((1, kv_heads, L, 128), dev, 2)
+    k[:, :, :64, 7] = -3e38
+    kv = filled(dev, k, v)
+    q = torch.zeros(1, heads, 128, dtype=torch.bfloat16, device=dev)
+    q[..., 7] = 3e38
+    q = q.flatten(1)
+    if columns == 0:
+        got = ops.attn_decode4(q, kv, 0, i32([0], dev), i32([L - 1], dev), heads, nsplit)
+    else:
+        got = ops.attn_prefill4(q, kv, 0, ops.kv4_prefill_plan([(0, 1, L - 1)], heads, kv_heads, dev, nsplit, columns * kv_heads // heads), heads)
+    vv = values(kv, 0)[1][:, 64:].repeat_interleave(heads // kv_heads, 0)
+    want, tol = vv.mean(1), 2.0 ** -8 * vv.mean(1).abs() + 2.0 ** -16 * vv.abs().mean(1)
+    U.assert_within(got, want.flatten()[None], tol.flatten()[None])

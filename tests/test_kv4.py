@@ -169,3 +169,18 @@ def test_cpu_tensors_are_refused(built_lib):
             call()
     with pytest.raises(TypeError):
         ops.kv4_read(object(), 0, i, i)
+
+
+def test_sizes_beyond_a_launch_or_63_bits_are_refused(built_lib):
+    """more than 2^32 threads; heads * layers whose offsets would wrap"""
+    lib, mem = built_lib, np.zeros(512, dtype=np.uint8)
+    p = (mem.ctypes.data + 255) // 256 * 256
+    lay = _lib.KvLayout(1, 8, 64, 128)
+    for S in (1 << 26, 0x7fffffff):
+        assert lib.lcc_kv4_read(p, 1, lay, 0, p, p, p, p, S, None) == -2
+        for fn in (lib.lcc_qk_norm_rope_kv_append_bf16, lib.lcc_qk_norm_rope_kv4_append):
+            assert fn(p, None, 0, None, None, None, 1e-6, p, p, p, p, None, p, 1, lay, 0, p, S, 64, None) == -2
+    for layers, heads in ((65535, 65535), (1 << 24, 2), (0x7fffffff, 1)):
+        assert lib.lcc_kv4_slot_bytes(_lib.KvLayout(layers, heads, 64, 128)) == 0
+        assert lib.lcc_kv4_read(p, 1, _lib.KvLayout(layers, heads, 64, 128), 0, p, p, p, p, 1, None) == -2
+    assert lib.lcc_kv4_slot_bytes(_lib.KvLayout(1 << 14, 1 << 10, 1 << 30, 128)) == 136 << 54
