@@ -376,13 +376,14 @@ int qk_norm_rope_append(const QkNormArgs& a, bool kv4, hipStream_t st) {
 // ------------------------------------------------------------------------------------------------------------------------------
 __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4Args a, const int32_t* __restrict__ tok_stream, const int32_t* __restrict__ tok_pos,
                                                        bf16_t* __restrict__ k_out, bf16_t* __restrict__ v_out, int rows) {
-  const int64_t item = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3);
-  if (item >= (int64_t)rows * a.n_kv_heads) return;
-  const int s = (int)(item / a.n_kv_heads), h = (int)(item - (int64_t)s * a.n_kv_heads), j = threadIdx.x & 7;
+  const int item = blockIdx.x * 32 + (threadIdx.x >> 3);
+  if (item >= rows * a.n_kv_heads) return;                                  // below 2^29
+  const int h = item / rows, s = item - h * rows, j = threadIdx.x & 7;
   const int slot = tok_stream[s], pos = tok_pos[s];
   // K: channels 16 j .. + 15.  V: bytes i = 8 z .. + 7 of group t, that is channels 32 t + 8 z .. + 7 and 32 t + 16 + 8 z .. + 7
   const int t = j >> 1, z = j & 1;
-  bf16_t *ko = k_out + (size_t)item * 128 + j * 16, *vo = v_out + (size_t)item * 128 + t * 32 + z * 8;
+  const size_t at = ((size_t)s * a.n_kv_heads + h) * 128;
+  bf16_t *ko = k_out + at + j * 16, *vo = v_out + at + t * 32 + z * 8;
   u32x4 k0 = {0, 0, 0, 0}, k1 = k0, v0 = k0, v1 = k0;
   if (slot >= 0 && slot < a.n_slots && pos >= 0 && pos < a.lmax) {
     const Kv4Layout lay{a.n_kv_heads, a.lmax};
@@ -631,13 +632,20 @@ static void kv4_combine(const float* ws_o, const float* ws_ml, bf16_t* out, cons
   else kv4_combine_kernel<4><<<dim3(items, n_tiles), dim3(256), 0, st>>>(ws_o, ws_ml, out, tile_q0, tile_nq, tile_rows, n_rows, n_q_heads, nsplit);
 }
 
+// Key splits of a decode step, by its blocks without any (rows x KV heads; a unit holds one) and the 32-key blocks of its longest row.  Measured (us, lengths spread over a quarter):
+//   Up to 32 key blocks: none; 28 / 4 heads, one row of 300 keys 5.0, in eight 6.3, of 1,000 7.7 / 6.8.
+//   Up to 32 blocks: a block for every unit.  One row of 32,000 keys 16 / 64 splits 16.6 / 10.2, 8 rows of 6,144 4 / 8 / 16 splits 13.7 / 11.1 / 12.0.
+//   Up to 64: as many, from 64 key blocks on: 16 rows of 1,100 keys 1 / 4 splits 7.6 / 8.4, of 2,400 12.8 / 10.3; eight from 192 on: of 6,144 14.4 / 14.6, of 16,000 33.5 / 28.7.
+//   Up to 192: eight, from 96 on.  Their lengths even out, and more waves load at a time: 40 rows of 2,400 keys 1 / 2 / 8 splits 13.6 / 16.5 / 16.6, of 6,144 34.0 / 36.2 / 30.1; 24 rows of 2,400
+//   13.0 / 12.7 / 12.7, of 6,144 26.2 / 20.4 / 18.0; 48 of 16,000 88.6 / 90.6 / 74.9.
+//   More: none.  56 rows of 6,144 keys 1 / 6 splits 41.1 / 40.3, 64 rows 45.2 / 44.9, of 2,400 15.8 / 20.4.
 int kv4_decode_splits(const int32_t* n_keys, int n, int n_kv_heads) {
   long most = 1;
   for (int i = 0; i < n; ++i) most = n_keys[i] > most ? n_keys[i] : most;
-  const long blocks = (most + 31) / 32, base = (long)(n > 0 ? n : 1) * n_kv_heads;
-  if (blocks <= 32) return 1;
-  const long k = std::min((256 + base - 1) / base, std::min(blocks / 4, 64L));
-  return (int)std::max(k, 1L);
+  const long keys = (most + 31) / 32, base = (long)(n > 0 ? n : 1) * n_kv_heads, units = (256 + base - 1) / base;
+  if (keys <= 32 || base > 192 || (base > 32 && keys < 64) || (base > 64 && keys < 96)) return 1;
+  const long k = base > 64 || (base > 32 && keys >= 192) ? 8 : units;
+  return (int)std::max(std::min(k, std::min(keys / 4, 64L)), 1L);
 }
 
 // eight waves where a block has all keys, four where they are split: 16 waves a unit in either case once there are blocks enough
