@@ -61,7 +61,10 @@ LCC_DEVICE unsigned scale_of(unsigned w) { return SEL < 3 ? w << (23 - 8 * SEL) 
 LCC_DEVICE u32x4 fp4_word(unsigned w, unsigned scale) { return (u32x4){fp4_pair<0>(w, scale), fp4_pair<1>(w, scale), fp4_pair<2>(w, scale), fp4_pair<3>(w, scale)}; }
 
 // ------------------------------------------------------------------------------------------------------------------------------
-// Norm, rotation, append.
+// Norm, rotation, append: every head row of a token is read once and written once (queries as bf16, keys and values into the cache).
+// Bound: up to some 400 rows the trip row -> tables -> cache (2.9 us for a row of 28 / 4 heads, 6 us for 386); 9,048 rows 45 us for 169 MB, 3.7 TB/s, where a copy of the same
+// bytes takes 34: the vector work of the norm and the eight roundings a pair (370 instructions a wave, 25 us by themselves) does not quite hide.  Blocks that stay and fetch their next item
+// ahead were no faster (46.5 us; 4 bits 35.9 against 37.8), nor four heads a lane group behind one load of the tables (57).
 // ------------------------------------------------------------------------------------------------------------------------------
 // scale byte of a group whose largest bf16 magnitude has the bits `a`
 LCC_DEVICE int kv4_exponent(int a) {
@@ -372,7 +375,8 @@ int qk_norm_rope_append(const QkNormArgs& a, bool kv4, hipStream_t st) {
 
 // ------------------------------------------------------------------------------------------------------------------------------
 // Read-back: row s = (slot, position) -> its keys and values [heads][128] in bf16; a row of no stream or position: zeros.  Eight lanes a (row, head), 16 channels
-// each.
+// each; rows run innermost, so that the bytes of V a wave gathers lie side by side where rows are neighbours (4,076 rows of 8 heads 8.1 -> 6.8 us; 21 MB).  Bound: two
+// trips, to the row's place and to its bytes.
 // ------------------------------------------------------------------------------------------------------------------------------
 __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4Args a, const int32_t* __restrict__ tok_stream, const int32_t* __restrict__ tok_pos,
                                                        bf16_t* __restrict__ k_out, bf16_t* __restrict__ v_out, int rows) {
@@ -416,7 +420,14 @@ int kv4_read(const Kv4Args& a, const int32_t* tok_stream, const int32_t* tok_pos
 // heads of the KV head.  S^T = K Q^T: operand A is 16 keys x 32 channels, a lane's 16 bytes of codes (one group of one key) its share of all four steps -- the
 // channels of step s are 8 s .. 8 s + 7 of each group, for Q alike.  Rows of the two key tiles are dealt so that a lane's eight scores are of the keys
 // 8 g .. 8 g + 7, which are the slots of its P operand: O^T += V^T P^T takes the probabilities from the softmax' registers and V's bytes as they lie.
+// The loads of a wave's next block go into the registers that the products have just left, K's first, so that either is waited for by a count while the other is in flight; 126
+// registers, 16 waves a unit (a second set of them: spills at that occupancy, and no gain at half of it).
+// Bound: 64 rows of 2,200 to 6,000 keys (28 / 4 heads) 32 us for 139 MB, 4.3 TB/s where a large copy moves 4.95 both ways together; the arithmetic alone takes 25 us.  One row of
+// 32,768 keys (64 / 8 heads, 64 splits) 10 us for 36 MB, of which some 4 are the launch and the first trip.
+// The same kernel takes tiles of a few rows of a chunk (CHUNK): its columns are then (row, head) pairs.
 // ------------------------------------------------------------------------------------------------------------------------------
+// The maximum that a softmax subtracts moves when a score passes it by more than 2^KV4_SLACK, not at every new one: sums and products scale alike, probabilities stay below
+// 2^8, and bf16's and fp32's relative steps are the same there.  Where it does not move, eight (chunks: 64) multiplications of O a block fall away.
 constexpr float KV4_SLACK = 8.f;
 struct Kv4Tile { u32x4 k[2], v[2], s[2]; unsigned ks[2]; };       // what a wave loads of a 32-key block: codes of two key tiles, of V, V's scales, K's
 struct Kv4Head { const uint8_t *kc, *vc, *ks, *vs; };              // a head's regions, wave-uniform: a lane's part of the addresses is 32 bits that never change
@@ -582,7 +593,8 @@ __global__ __launch_bounds__(NW * 64, 4) void attn_rows_kv4_kernel(Kv4Args a, Kv
 }
 
 // Joins the key splits of a (row, head): sums weighted by 2^(m - max), one rounding.  A half-wave reads a split's 128 channels at a time; W waves share a (row, head).
-// blockIdx.y: a tile, or (tiles null) a row.
+// blockIdx.y: a tile, or (tiles null) a row.  All loads of a (row, head) are in flight before the first weight is known; a trip's time otherwise: 64 splits of 64 heads 3.6 us,
+// of 17 rows x 28 4.3 us (15.8 MB), five of 386 rows 7.6 us (28 MB, 3.7 TB/s).  In one wave (W = 1) to 8 splits, in four beyond: those have more to load than registers.
 template <int W>
 __global__ __launch_bounds__(256) void kv4_combine_kernel(const float* __restrict__ ws_o, const float* __restrict__ ws_ml, bf16_t* __restrict__ out,
                                                           const int32_t* __restrict__ tile_q0, const int32_t* __restrict__ tile_nq, int tile_rows, int n_rows, int n_q_heads,
@@ -676,6 +688,12 @@ int attn_decode_kv4(const Kv4Args& a, const bf16_t* q, const int32_t* slots, con
 // Attention of chunks: tiles of up to 256 / G consecutive new rows of one stream, their (row, head) pairs the 8 x 32 columns of a block's waves.  The
 // block turns 64 keys at a time into bf16 in LDS (each thread eight bytes of K and of V) and every wave multiplies them: S^T = K Q^T and
 // O^T += V^T P^T on 32x32x16, K's rows read in the order (bits 2 and 3 swapped) that leaves a lane the scores of the keys its P operand wants.
+// Conversion once a block and stage is what LDS is for: 8 KB of codes become 32 KB that all waves read, in images whose 16-byte chunks are permuted so that neither the reads (16 lanes at
+// a time) nor the writes (8) meet in a bank (no conflicts counted).
+// Bound: eight chunks of ~340 rows on ~5,000 keys 243 us, 0.86 PFLOP/s where a large matrix product reaches 1.20: of a wave's 64-key stage 1,024 clocks are matrix instructions and some 950
+// vector ones (conversion, softmax), and the two waves of a SIMD overlap them by little (matrix units busy half of the time).  Other orders of the stage, pinned or with
+// priorities, were no faster (159 -> 170 us for 386 rows unsplit); products in the 4-bit type itself, with queries in parts of 8 bits, sum to 2^-13.5 only and were not taken.
+// Few rows: 17 rows of 28 / 4 heads on 26,800 keys 21 us, a third of it the 64 splits' partials (15.8 MB).
 // ------------------------------------------------------------------------------------------------------------------------------
 constexpr int KV4_STAGE = 64, KV4_KB = KV4_STAGE * 256, KV4_VB = 128 * KV4_STAGE * 2, KV4_LDS = 2 * (KV4_KB + KV4_VB);
 template <int U> struct Kv4Stage { u32x2 k[U], v[U], s[U]; unsigned ks[U]; };
