@@ -539,6 +539,8 @@ __global__ __launch_bounds__(NW * 64, 4) void attn_rows_kv4_kernel(Kv4Args a, Kv
       float p[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) { p[e] = __builtin_amdgcn_exp2f(fmaf(sc[e >> 2][e & 3], scale_log2e, -mu)); l += p[e]; }
+      // The products take probabilities in bf16, as the bf16 cache's attention does (l sums them unrounded):
+      // each off by half a step at most, 2^-8 of itself, and so the result by 2^-8 of the weighted mean of |V|.
       // A converted byte is a pair (channel i, channel 16 + i) of one key, two slots of the operand: against (p, 0) it is channel i's product, against (0, p) the other's.
       u32x4 pl[2], ph[2];
 #pragma unroll
@@ -965,7 +967,7 @@ int kv4_prefill_plan(const int32_t* n_new, const int32_t* past, int n, int n_q_h
     const int height = columns / G, keys = columns == 16 ? 32 : KV4_STAGE;
     long tiles = 0, total = 0, longest = 0;                                 // stages (blocks of 32 keys) of a KV head
     for (int i = 0; i < n; ++i) {
-      const long count = (n_new[i] + height - 1) / height;
+      const long count = ((long)n_new[i] + height - 1) / height;
       tiles += count;
       for (long z = 0; z < std::min(count, 64L); ++z) {                     // of many tiles 64 spread over the stream stand for all
         const long t = count <= 64 ? z : z * count / 64, st = (past[i] + std::min<long>(n_new[i], (t + 1) * height) + keys - 1) / keys;

@@ -618,3 +618,53 @@ def test_keys_whose_scores_are_minus_infinity(dev, columns, nsplit):
     vv = values(kv, 0)[1][:, 64:].repeat_interleave(heads // kv_heads, 0)
     want, tol = vv.mean(1), 2.0 ** -8 * vv.mean(1).abs() + 2.0 ** -16 * vv.abs().mean(1)
     U.assert_within(got, want.flatten()[None], tol.flatten()[None])
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("heads,kv_heads", [(28, 4), (64, 8), (30, 2), (31, 1), (0, 3), (5, 5)])
+@pytest.mark.parametrize("rows,slabs", [(513, 0), (700, 2)])
+def test_append_in_one_call_as_in_many(dev, bits, heads, kv_heads, rows, slabs):
+    """rows enough for V to go by windows, against the same rows a hundred at a time: the same queries and the same cache, bit for bit"""
+    from livecc_amd import ops
+    lmax, width = 416, (heads + 2 * kv_heads) * 128
+    src = rand((slabs, rows, width), dev, 1).float() if slabs else rand((rows, width), dev, 1, 2.0)
+    cos, sin = tables(range(rows), dev)
+    qn, kn = rand((128,), dev, 2), rand((128,), dev, 3)
+    half = rows // 2 + 9
+    st = i32([1] * half + [0] * (rows - half), dev)
+    pos = i32([3 + r for r in range(half)] + list(range(rows - half)), dev)
+    out = []
+    for step in (rows, 100):
+        kv = (ops.Kv4Arena if bits == 4 else ops.KvArena)(2, 1, kv_heads, lmax, dev)
+        q = [ops.qk_norm_rope_kv_append(None if slabs else src[i:i + step], cos[i:i + step], sin[i:i + step], st[i:i + step], pos[i:i + step], kv, 0, heads, q_norm=qn, k_norm=kn,
+                                        partial=src[:, i:i + step].contiguous() if slabs else None) for i in range(0, rows, step)]
+        out.append((torch.cat(q), kv.buf))
+    assert torch.equal(out[0][0], out[1][0]) and torch.equal(out[0][1], out[1][1])
+
+
+def test_decode_of_many_rows_of_few_slots(dev):
+    """600 rows, most of them of the same slots: each as alone"""
+    from livecc_amd import ops
+    heads, kv_heads, L = 6, 2, 160
+    kv = filled(dev, rand((3, kv_heads, L, 128), dev, 1), rand((3, kv_heads, L, 128), dev, 2))
+    slots = i32([(7 * r) % 3 if r % 11 else -1 for r in range(600)], dev)
+    lens, q = i32([159, 64, 7], dev), rand((600, heads * 128), dev, 3)
+    for nsplit in (1, 2):
+        got = ops.attn_decode4(q, kv, 0, slots, lens, heads, nsplit)
+        for i in (0, 1, 2, 22, 301, 599):
+            assert torch.equal(got[i:i + 1], ops.attn_decode4(q[i:i + 1].contiguous(), kv, 0, slots[i:i + 1].contiguous(), lens, heads, nsplit)), i
+
+
+def test_inputs_that_would_record_a_gradient_are_refused(dev):
+    from livecc_amd import ops
+    heads, kv_heads = 4, 2
+    kv = ops.Kv4Arena(1, 1, kv_heads, 64, dev)
+    qkv, at = rand((1, 8 * 128), dev, 1).requires_grad_(), i32([0], dev)
+    cos, sin = tables([0], dev)
+    q = rand((1, heads * 128), dev, 2).requires_grad_()
+    for call in (lambda: ops.qk_norm_rope_kv_append(qkv, cos, sin, at, at, kv, 0, heads), lambda: ops.attn_decode4(q, kv, 0, at, at, heads),
+                 lambda: ops.attn_prefill4(q, kv, 0, [(0, 1, 0)], heads)):
+        with pytest.raises(RuntimeError):
+            call()
+        with torch.no_grad():
+            call()
