@@ -62,9 +62,10 @@ LCC_DEVICE u32x4 fp4_word(unsigned w, unsigned scale) { return (u32x4){fp4_pair<
 
 // ------------------------------------------------------------------------------------------------------------------------------
 // Norm, rotation, append: every head row of a token is read once and written once (queries as bf16, keys and values into the cache).
-// Bound: up to some 400 rows the trip row -> tables -> cache (2.9 us for a row of 28 / 4 heads, 6 us for 386); 9,048 rows 45 us for 169 MB, 3.7 TB/s, where a copy of the same
-// bytes takes 34: the vector work of the norm and the eight roundings a pair (370 instructions a wave, 25 us by themselves) does not quite hide.  Blocks that stay and fetch their next item
-// ahead were no faster (46.5 us; 4 bits 35.9 against 37.8), nor four heads a lane group behind one load of the tables (57).
+// Bound: up to some 400 rows the trips to a row, its place and the cache (2.7 us for a row of 28 / 4 heads, 4.5 us for 386); 9,048 rows 36.8 us for 169 MB, 4,076 rows of 64 / 8 heads into
+// 4 bits 32 us for 155 MB, 4.6-4.8 TB/s, where a copy of the same bytes takes 34 and 31: the vector work (the norm and eight roundings a pair, some 350 instructions a wave, 25 us by
+// themselves) hides behind the memory as long as all loads of a lane are in flight before the first wait (one after the other: 3 us more) and V is stored by whole octets.  Blocks that stay
+// and fetch their next item ahead were no faster, nor four heads a lane group behind one load of the tables; sums in 32 bits would save nothing.
 // ------------------------------------------------------------------------------------------------------------------------------
 // scale byte of a group whose largest bf16 magnitude has the bits `a`
 LCC_DEVICE int kv4_exponent(int a) {
@@ -89,43 +90,57 @@ LCC_DEVICE int max_bits(const u32x4& x) {
   for (int d = 0; d < 4; ++d) { const int lo = x[d] & 0x7fff, hi = x[d] >> 16 & 0x7fff; a = max(a, max(lo, hi)); }
   return a;
 }
+// lane ^ X of 32: on the LDS crossbar, whose pattern is a constant (a lane's address would be vector work, which large calls have no room for; moves of the vector unit: 45.5 -> 47.4 us
+// for 9,048 rows)
+template <int X> LCC_DEVICE int lane_xor(int x) { return __builtin_amdgcn_ds_swizzle(x, X << 10 | 0x1f); }
+template <int X> LCC_DEVICE double lane_xor(double x) {
+  const unsigned long long u = __builtin_bit_cast(unsigned long long, x);
+  const unsigned lo = lane_xor<X>((int)(unsigned)u), hi = lane_xor<X>((int)(unsigned)(u >> 32));
+  return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
+}
 // over the four lanes that hold a group
 LCC_DEVICE int max4(int a) {
-  a = max(a, __shfl_xor(a, 1, 64));
-  return max(a, __shfl_xor(a, 2, 64));
+  a = max(a, lane_xor<1>(a));
+  return max(a, lane_xor<2>(a));
 }
 
-// eight channels of a row: bf16, or bf16(sum of the slabs + bias)
-LCC_DEVICE void row8(const QkNormArgs& a, int s, int col, float* v) {
-  const int ld = (a.n_q_heads + 2 * a.n_kv_heads) * 128;
+// A lane's 16 channels of a head (c0 .. + 7, c0 + 64 .. + 71) of a row: bf16, or bf16(sum of the slabs + bias).  rows * heads fits 31 bits.
+LCC_DEVICE void row16(const QkNormArgs& a, int s, int head, int c0, float (&x1)[8], float (&x2)[8]) {
+  const int heads = a.n_q_heads + 2 * a.n_kv_heads;
   if (a.partial == nullptr) {
-    const u32x4 x = ld16(a.qkv + (size_t)s * ld + col);
+    const bf16_t* p = a.qkv + ((size_t)(unsigned)(s * heads + head) << 7) + c0;
+    const u32x4 y1 = ld16(p), y2 = ld16(p + 64);
 #pragma unroll
-    for (int d = 0; d < 4; ++d) { v[2 * d] = lo2f(x[d]); v[2 * d + 1] = hi2f(x[d]); }
+    for (int d = 0; d < 4; ++d) { x1[2 * d] = lo2f(y1[d]); x1[2 * d + 1] = hi2f(y1[d]); x2[2 * d] = lo2f(y2[d]); x2[2 * d + 1] = hi2f(y2[d]); }
     return;
   }
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = 0.f;
-  for (int sp = 0; sp < a.nsplit; ++sp) {
-    const float* p = a.partial + ((size_t)sp * a.rows + s) * ld + col;
-    const f32x4 x = *reinterpret_cast<const f32x4*>(p), y = *reinterpret_cast<const f32x4*>(p + 4);
+  for (int half = 0; half < 2; ++half) {
+    float(&v)[8] = half ? x2 : x1;
+    const int col = head * 128 + c0 + half * 64;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) { v[e] += x[e]; v[4 + e] += y[e]; }
+    for (int e = 0; e < 8; ++e) v[e] = 0.f;
+    for (int sp = 0; sp < a.nsplit; ++sp) {
+      const float* p = a.partial + ((size_t)sp * a.rows + s) * heads * 128 + col;
+      const f32x4 x = *reinterpret_cast<const f32x4*>(p), y = *reinterpret_cast<const f32x4*>(p + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { v[e] += x[e]; v[4 + e] += y[e]; }
+    }
+    const u32x4 b = a.bias != nullptr ? ld16(a.bias + col) : (u32x4){0, 0, 0, 0};
+#pragma unroll
+    for (int d = 0; d < 4; ++d) { v[2 * d] = rbf(v[2 * d] + lo2f(b[d])); v[2 * d + 1] = rbf(v[2 * d + 1] + hi2f(b[d])); }
   }
-  const u32x4 b = a.bias != nullptr ? ld16(a.bias + col) : (u32x4){0, 0, 0, 0};
-#pragma unroll
-  for (int d = 0; d < 4; ++d) { v[2 * d] = rbf(v[2 * d] + lo2f(b[d])); v[2 * d + 1] = rbf(v[2 * d + 1] + hi2f(b[d])); }
 }
 
 // RMS norm of a head's 128 channels over its eight lanes, with the model's rounding points: bf16(w bf16(x r)).  The mean square and its root are formed in 64
 // bits and r is rounded once: keys are quantised behind this, and codes must not depend on the order of a sum.
-LCC_DEVICE void head_norm(float (&x1)[8], float (&x2)[8], const bf16_t* w, int c0, float eps) {
-  const u32x4 w1 = ld16(w + c0), w2 = ld16(w + c0 + 64);
+LCC_DEVICE void head_norm(float (&x1)[8], float (&x2)[8], const u32x4& w1, const u32x4& w2, float eps) {
   double ss = 0.0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) { ss = fma((double)x1[e], (double)x1[e], ss); ss = fma((double)x2[e], (double)x2[e], ss); }
-#pragma unroll
-  for (int o = 1; o < 8; o <<= 1) ss += __shfl_xor(ss, o, 64);
+  ss += lane_xor<1>(ss);
+  ss += lane_xor<2>(ss);
+  ss += lane_xor<4>(ss);
   const double m = ss * (1.0 / 128) + (double)eps;
   double r = __builtin_amdgcn_rsq(m);
   if (m < __builtin_inf()) r = fma(0.5 * r, fma(-m * r, r, 1.0), r);        // the unit's result is good to about 2^-28; one step squares that
@@ -140,9 +155,10 @@ LCC_DEVICE void head_norm(float (&x1)[8], float (&x2)[8], const bf16_t* w, int c
   }
 }
 
-// From so many rows on V goes by windows: 1,131 rows of 28 / 4 heads 11.5 -> 9.0 us (4 bits 9.3 -> 8.3), 9,048 rows 62 -> 48 (46.6 -> 42.8); 386 rows 5.9 either way, 100 rows 4.4
-// against 5.1
-constexpr int KV4_WINDOW_ROWS = 512;
+// From so many rows on V goes by windows (us, without and with; 28 / 4 heads unless said).  A chunk of 128 rows 4.4 / 3.8 (4 bits 4.5 / 4.3), of 386 5.8 / 4.5 (5.5 / 4.9), of 1,131 10.7 / 7.0
+// (8.4 / 7.0); 600 tokens of as many streams, no octet among them, 8.7 / 8.5 (6.3 / 6.6).  It costs most with 64 / 8 heads in 4 bits: 386 rows 6.3 / 6.7, 600 tokens 7.8 / 9.7.  Below, one
+// wave's row is as quick: 64 rows 4.2 / 3.7 (4.5 / 4.2), and batches of single tokens are of that size.
+constexpr int KV4_WINDOW_ROWS = 128;
 // Where a row's keys and values go: its slot and position, slot -1 for a row of no stream or no position.
 LCC_DEVICE void row_place(const QkNormArgs& a, int s, int& slot, int& pos) {
   slot = a.tok_stream[s];
@@ -156,7 +172,7 @@ LCC_DEVICE void v_codes(const u32x4& r1, const u32x4& r2, int j, u32x2& bytes, i
   const int e1 = kv4_exponent(max4(max_bits(r1))), e2 = kv4_exponent(max4(max_bits(r2)));
   const unsigned w1 = fp4_of(r1, e1), w2 = fp4_of(r2, e2);
   const bool up = (j & 2) != 0;
-  const unsigned mine = up ? w2 : w1, other = __shfl_xor(up ? w1 : w2, 2, 64), lo = up ? other : mine, hi = up ? mine : other;
+  const unsigned mine = up ? w2 : w1, other = lane_xor<2>((int)(up ? w1 : w2)), lo = up ? other : mine, hi = up ? mine : other;
   t = up ? 2 + (j >> 2) : j >> 2;
   e = up ? e2 : e1;
 #pragma unroll
@@ -167,103 +183,110 @@ LCC_DEVICE void v_codes(const u32x4& r1, const u32x4& r2, int j, u32x2& bytes, i
   }
 }
 // 16 channels of a row: a lane's r1, r2
-LCC_DEVICE void row_pairs(const QkNormArgs& a, int s, int col, u32x4& r1, u32x4& r2) {
+LCC_DEVICE void row_pairs(const QkNormArgs& a, int s, int head, int c0, u32x4& r1, u32x4& r2) {
   float x1[8], x2[8];
-  row8(a, s, col, x1);
-  row8(a, s, col + 64, x2);
+  row16(a, s, head, c0, x1, x2);
 #pragma unroll
   for (int d = 0; d < 4; ++d) { r1[d] = pack2(x1[2 * d], x1[2 * d + 1]); r2[d] = pack2(x2[2 * d], x2[2 * d + 1]); }
 }
 
-// V of 32 consecutive rows of a KV head, a block: V lies position-innermost, so rows are turned in LDS.  Where the rows are consecutive positions of one stream (a chunk
-// but for its ends) each run of eight aligned positions is one store of a channel (16 bytes of bf16; 4 bits: 8 of a channel pair), else positions are stored one by one.
+// V of 32 consecutive rows of a KV head, a block: V lies position-innermost, so rows are turned in LDS.  Eight rows that are the eight positions of an aligned octet of one stream are one
+// store of a channel (16 bytes of bf16; 4 bits: 8 of a byte): the block in whose window they begin takes the rows behind its window along and writes them all.  Rows of no such octet (ends
+// of a chunk, single tokens) are stored one by one, rows of an octet that began before the window not at all.
+constexpr int KV4_V_ROWS = 39;                                              // a window and what an octet may take behind it
+template <bool KV4> constexpr int KV4_V_PITCH = KV4 ? 68 : 260;             // bytes of a row: 64 code bytes [t][i] and 4 scales, or 128 bf16 (+ 4: rows on other banks)
 template <bool KV4>
 LCC_DEVICE void append_v_window(const QkNormArgs& a, int h, int r0, unsigned char* lds) {
-  constexpr int PITCH = KV4 ? 68 : 260;                                     // bytes of a row: 64 code bytes [t][i] and 4 scales, or 128 bf16 (+ 4: rows on other banks)
-  const int tid = threadIdx.x, row = tid >> 3, j = tid & 7, n = min(32, a.rows - r0), lane = tid & 63;
+  constexpr int PITCH = KV4_V_PITCH<KV4>;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), j = tid & 7, head = a.n_q_heads + a.n_kv_heads + h;
   u32x4 r1, r2;
-  row_pairs(a, r0 + min(row, n - 1), (a.n_q_heads + a.n_kv_heads + h) * 128 + j * 8, r1, r2);
-  int slot, pos;
-  row_place(a, r0 + min(lane & 31, n - 1), slot, pos);
-  unsigned char* at = lds + row * PITCH;
-  if (KV4) {
-    u32x2 w; int t, e;
-    v_codes(r1, r2, j, w, t, e);
-    *reinterpret_cast<unsigned*>(at + t * 16 + (j & 1) * 8) = w[0];
-    *reinterpret_cast<unsigned*>(at + t * 16 + (j & 1) * 8 + 4) = w[1];
-    if ((j & 1) == 0) at[64 + t] = (unsigned char)e;
-  } else {
+  row_pairs(a, min(r0 + (tid >> 3), a.rows - 1), head, j * 8, r1, r2);
+  auto stage = [&](int row) {
+    unsigned char* at = lds + row * PITCH;
+    if (KV4) {
+      u32x2 w; int t, e;
+      v_codes(r1, r2, j, w, t, e);
+      *reinterpret_cast<unsigned*>(at + t * 16 + (j & 1) * 8) = w[0];
+      *reinterpret_cast<unsigned*>(at + t * 16 + (j & 1) * 8 + 4) = w[1];
+      if ((j & 1) == 0) at[64 + t] = (unsigned char)e;
+    } else {
 #pragma unroll
-    for (int d = 0; d < 4; ++d) { *reinterpret_cast<unsigned*>(at + j * 16 + 4 * d) = r1[d]; *reinterpret_cast<unsigned*>(at + 128 + j * 16 + 4 * d) = r2[d]; }
+      for (int d = 0; d < 4; ++d) { *reinterpret_cast<unsigned*>(at + j * 16 + 4 * d) = r1[d]; *reinterpret_cast<unsigned*>(at + 128 + j * 16 + 4 * d) = r2[d]; }
+    }
+  };
+  // lane i has row r0 - 7 + i: 46 rows, those of every octet that reaches into the window
+  int slot = -1, pos = 0;
+  const int mine = r0 - 7 + lane;
+  if (lane < 46 && mine >= 0 && mine < a.rows) row_place(a, mine, slot, pos);
+  const unsigned long long arena = slot >= 0 ? (unsigned long long)a.kv_base[slot] : 0;
+  const int before = __shfl_up(slot, 1, 64), pos_before = __shfl_up(pos, 1, 64);
+  const unsigned long long next = __ballot(lane > 0 && slot >= 0 && slot == before && pos == pos_before + 1);       // rows that continue the one before
+  const int first = lane - (pos & 7);                                       // of the row's octet
+  const bool whole = slot >= 0 && first >= 0 && ((next >> (max(first, 0) + 1)) & 0x7f) == 0x7f, window = lane >= 7 && lane < 39;
+  unsigned long long octets = __ballot(window && whole && first == lane), singles = __ballot(window && slot >= 0 && !whole);
+  stage(tid >> 3);
+  if ((octets >> 32) != 0 && tid < 56) {                                    // the last octet ends behind the window
+    row_pairs(a, min(r0 + 32 + (tid >> 3), a.rows - 1), head, j * 8, r1, r2);
+    stage(32 + (tid >> 3));
   }
-  const int slot0 = __builtin_amdgcn_readfirstlane(slot), pos0 = __builtin_amdgcn_readfirstlane(pos);
-  const bool chunk = __all((lane & 31) >= n || (slot0 >= 0 && slot == slot0 && pos == pos0 + (lane & 31)));
   __syncthreads();
   const Kv4Layout lay{a.n_kv_heads, a.lmax};
   const size_t kv = (size_t)a.n_kv_heads * a.lmax * 128;
-  auto base_of = [&](int sl) -> uint8_t* {
-    return KV4 ? (uint8_t*)a.kv_base[sl] + (size_t)a.layer * lay.layer_bytes() : (uint8_t*)((bf16_t*)a.kv_base[sl] + ((size_t)a.layer * 2 + 1) * kv + (size_t)h * a.lmax * 128);
+  auto base_of = [&](int o) -> uint8_t* {                                   // of lane o's row
+    uint8_t* at = (uint8_t*)((unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)(arena >> 32), o) << 32 | (unsigned)__builtin_amdgcn_readlane((int)(unsigned)arena, o));
+    return KV4 ? at + (size_t)a.layer * lay.layer_bytes() : (uint8_t*)((bf16_t*)at + ((size_t)a.layer * 2 + 1) * kv + (size_t)h * a.lmax * 128);
   };
-  // a thread turns one word of eight rows: four bytes' units of eight positions (code bytes 4 (u mod 4) .. + 3 of group u / 4; u = 16: the scales), or a pair of channels
-  constexpr int UNITS = KV4 ? 17 : 64;
-  const int shift = chunk ? pos0 & 7 : 0, octets = (shift + n + 7) / 8;
-  for (int i = tid; i < octets * UNITS; i += 256) {
-    const int oct = i / UNITS, u = i - oct * UNITS;
-    const int first = oct * 8 - shift, e0 = max(0, -first), e1 = min(8, n - first);         // rows first + e0 .. first + e1 - 1 of the window
-    unsigned x[8];
+  auto place4 = [&](uint8_t* base, int ps, int b) -> uint8_t* {             // byte b of a row: codes (t, i), from 64 on scales
+    return b < 64 ? base + lay.v_codes(h) + (size_t)(ps >> 5) * 2048 + ((ps & 31) >> 3) * 512 + (b & 15) * 32 + (b >> 4) * 8 + (ps & 7)
+                  : base + lay.v_scales(h) + (size_t)(ps >> 5) * 128 + ((ps & 31) >> 3) * 32 + (b - 64) * 8 + (ps & 7);
+  };
+  auto place16 = [&](uint8_t* base, int ps, int c) { return (bf16_t*)base + ((size_t)(ps >> 5) * 128 + c) * 32 + (ps & 31); };
+  // up to four octets, a wave each; singles in turn
+  for (int i = 0; i < wave; ++i) { octets &= octets - 1; singles &= singles - 1; }
+  if (octets != 0) {
+    const int o = __builtin_ctzll(octets), ps = __builtin_amdgcn_readlane(pos, o);
+    uint8_t* base = base_of(o);
+    const unsigned char* at = lds + (o - 7) * PITCH;
+    if (KV4) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = *reinterpret_cast<const unsigned*>(lds + min(max(first + e, 0), 31) * PITCH + u * 4);
-    auto place4 = [&](uint8_t* base, int ps, int z) -> uint8_t* {           // byte z of the word
-      return u < 16 ? base + lay.v_codes(h) + (size_t)(ps >> 5) * 2048 + ((ps & 31) >> 3) * 512 + ((u & 3) * 4 + z) * 32 + (u >> 2) * 8 + (ps & 7)
-                    : base + lay.v_scales(h) + (size_t)(ps >> 5) * 128 + ((ps & 31) >> 3) * 32 + z * 8 + (ps & 7);
-    };
-    auto place16 = [&](uint8_t* base, int ps) { return (bf16_t*)base + ((size_t)(ps >> 5) * 128 + u * 2) * 32 + (ps & 31); };
-    if (chunk && e1 - e0 == 8) {
-      uint8_t* base = base_of(slot0);
-      if (KV4) {
+      for (int b = lane; b < 68; b += 64) {                                 // a byte of the rows
+        u32x2 w = {0, 0};
 #pragma unroll
-        for (int z = 0; z < 4; ++z) {
-          u32x2 w;
-#pragma unroll
-          for (int d = 0; d < 2; ++d) {
-            const unsigned sel = 0x0c0c0400u + 0x101u * z;                  // byte z of either operand
-            const unsigned ab = __builtin_amdgcn_perm(x[4 * d + 1], x[4 * d], sel), cd = __builtin_amdgcn_perm(x[4 * d + 3], x[4 * d + 2], sel);
-            w[d] = __builtin_amdgcn_perm(cd, ab, 0x05040100u);
-          }
-          st8(place4(base, pos0 + first, z), w);
-        }
-      } else {
-        u32x4 lo, hi;
-#pragma unroll
-        for (int d = 0; d < 4; ++d) { lo[d] = __builtin_amdgcn_perm(x[2 * d + 1], x[2 * d], 0x05040100u); hi[d] = __builtin_amdgcn_perm(x[2 * d + 1], x[2 * d], 0x07060302u); }
-        bf16_t* dst = place16(base, pos0 + first);
-        st16(dst, lo); st16(dst + 32, hi);
+        for (int e = 0; e < 8; ++e) w[e >> 2] |= (unsigned)at[e * PITCH + b] << (8 * (e & 3));
+        st8(place4(base, ps, b), w);
       }
-    } else {
+    } else {                                                                // a pair of channels
+      u32x4 lo, hi;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {                                         // each row to its own place
-        int sl = chunk ? slot0 : -1, ps = pos0 + first + e;
-        if (e < e0 || e >= e1) continue;
-        if (!chunk) row_place(a, r0 + first + e, sl, ps);
-        if (sl < 0) continue;
-        uint8_t* base = base_of(sl);
-        if (KV4) {
-#pragma unroll
-          for (int z = 0; z < 4; ++z) *place4(base, ps, z) = (uint8_t)(x[e] >> (8 * z));
-        } else {
-          bf16_t* dst = place16(base, ps);
-          dst[0] = (bf16_t)x[e]; dst[32] = (bf16_t)(x[e] >> 16);
-        }
+      for (int d = 0; d < 4; ++d) {
+        const unsigned x = *reinterpret_cast<const unsigned*>(at + 2 * d * PITCH + lane * 4), y = *reinterpret_cast<const unsigned*>(at + (2 * d + 1) * PITCH + lane * 4);
+        lo[d] = __builtin_amdgcn_perm(y, x, 0x05040100u); hi[d] = __builtin_amdgcn_perm(y, x, 0x07060302u);
       }
+      bf16_t* dst = place16(base, ps, lane * 2);
+      st16(dst, lo); st16(dst + 32, hi);
     }
+  }
+  while (singles != 0) {
+    const int o = __builtin_ctzll(singles), ps = __builtin_amdgcn_readlane(pos, o);
+    uint8_t* base = base_of(o);
+    const unsigned char* at = lds + (o - 7) * PITCH;
+    if (KV4) {
+      for (int b = lane; b < 68; b += 64) *place4(base, ps, b) = at[b];
+    } else {
+      const unsigned x = *reinterpret_cast<const unsigned*>(at + lane * 4);
+      bf16_t* dst = place16(base, ps, lane * 2);
+      dst[0] = (bf16_t)x; dst[32] = (bf16_t)(x >> 16);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) singles &= singles - 1;
   }
 }
 
 // Eight lanes a (row, head), lane j with channels 8 j .. + 7 and 64 + 8 j .. + 7: the rotation's pairs and, four lanes each, two groups of the 4-bit format
-// (2 shuffles a group, 3 for the norm).  WINDOWS: every v_every-th block takes V of a window of rows, the others queries and keys.
+// (2 exchanges a group, 3 for the norm).  WINDOWS: every v_every-th block takes V of a window of rows, the others queries and keys.
 template <bool KV4, bool WINDOWS>
 __global__ __launch_bounds__(256) void qk_norm_rope_append_kernel(QkNormArgs a, int v_blocks, int v_every) {
-  __shared__ __attribute__((aligned(16))) unsigned char lds[WINDOWS ? 32 * (KV4 ? 68 : 260) : 16];
+  __shared__ __attribute__((aligned(16))) unsigned char lds[WINDOWS ? KV4_V_ROWS * KV4_V_PITCH<KV4> : 16];
   int block = (int)blockIdx.x;
   if (WINDOWS) {
     const int w = block / v_every;
@@ -287,15 +310,18 @@ __global__ __launch_bounds__(256) void qk_norm_rope_append_kernel(QkNormArgs a, 
   const int j = threadIdx.x & 7, c0 = j * 8, kind = head < a.n_q_heads ? 0 : head < a.n_q_heads + a.n_kv_heads ? 1 : 2;
   const int h = kind == 0 ? head : head - a.n_q_heads - (kind - 1) * a.n_kv_heads;
   int slot = 0, pos = 0;
-  if (kind > 0) row_place(a, s, slot, pos);
   u32x4 r1, r2;
   if (kind < 2) {
-    float x1[8], x2[8];
-    row8(a, s, head * 128 + c0, x1);
-    row8(a, s, head * 128 + 64 + c0, x2);
-    const u32x4 cq = ld16(a.cos + (size_t)s * 64 + c0), sq = ld16(a.sin + (size_t)s * 64 + c0);
+    // all loads ahead of the first wait
     const bf16_t* w = kind ? a.k_norm : a.q_norm;
-    if (w != nullptr) head_norm(x1, x2, w, c0, a.eps);
+    const u32x4 cq = ld16(a.cos + (size_t)s * 64 + c0), sq = ld16(a.sin + (size_t)s * 64 + c0);
+    u32x4 w1 = {0, 0, 0, 0}, w2 = w1;
+    if (w != nullptr) { w1 = ld16(w + c0); w2 = ld16(w + c0 + 64); }
+    float x1[8], x2[8];
+    asm volatile("" ::: "memory");
+    row16(a, s, head, c0, x1, x2);
+    if (kind > 0) row_place(a, s, slot, pos);
+    if (w != nullptr) head_norm(x1, x2, w1, w2, a.eps);
 #pragma unroll
     for (int d = 0; d < 4; ++d) {
       float p[4], q[4];                                                     // the four products of channels 2 d, 2 d + 1 and their partners, rounded
@@ -309,11 +335,14 @@ __global__ __launch_bounds__(256) void qk_norm_rope_append_kernel(QkNormArgs a, 
       r1[d] = pack2(p[0] + p[2], p[1] + p[3]); r2[d] = pack2(q[0] + q[2], q[1] + q[3]);
     }
     if (kind == 0) {
-      bf16_t* q = a.q_out + ((size_t)s * a.n_q_heads + h) * 128 + c0;
+      bf16_t* q = a.q_out + ((size_t)(unsigned)(s * a.n_q_heads + h) << 7) + c0;
       st16(q, r1); st16(q + 64, r2);
       return;
     }
-  } else row_pairs(a, s, head * 128 + c0, r1, r2);
+  } else {
+    row_pairs(a, s, head, c0, r1, r2);
+    row_place(a, s, slot, pos);
+  }
   if (slot < 0) return;
   if (!KV4) {
     bf16_t* base = (bf16_t*)a.kv_base[slot] + ((size_t)(a.layer * 2 + kind - 1) * a.n_kv_heads + h) * a.lmax * 128;

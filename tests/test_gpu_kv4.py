@@ -149,7 +149,7 @@ def test_append_at_kv_len_and_rows_of_no_stream(dev, bits):
 @pytest.mark.parametrize("rows", [130, 600])
 @pytest.mark.parametrize("how", ["tokens of many streams", "a chunk with gaps", "one chunk", "two chunks", "a chunk that leaves the arena"])
 def test_append_of_many_rows(dev, bits, rows, how):
-    """from 512 rows on V goes by windows of 32 rows, whole runs of eight positions where a window is one chunk, rows one by one where it is not"""
+    """V by windows of 32 rows: whole octets of positions where the rows are consecutive, rows one by one where they are not"""
     from livecc_amd import ops
     heads, kv_heads, lmax = 2, 2, 640
     if how == "tokens of many streams":
@@ -668,3 +668,39 @@ def test_inputs_that_would_record_a_gradient_are_refused(dev):
             call()
         with torch.no_grad():
             call()
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("seed", range(6))
+def test_append_of_runs_of_all_lengths(dev, bits, seed):
+    """Runs of 1 to 40 consecutive positions of shuffled slots, rows of no stream between them: octets begin, end and break anywhere in a window and across two.  In one call as
+    in calls of few rows."""
+    import random
+    from livecc_amd import ops
+    heads, kv_heads, n, lmax = 3, 1, 5, 224
+    rng = random.Random(seed)
+    runs, left = [], []
+    for slot in range(n):
+        p = rng.choice((0, 1, 7, 8))
+        while p < lmax:
+            k = min(rng.choice((1, 2, 7, 8, 9, 16, 23, 40)), lmax - p)
+            runs.append([(slot, p + r) for r in range(k)])
+            p += k + rng.choice((0, 0, 1, 8))
+    rng.shuffle(runs)
+    for run in runs:
+        left += run + [(-1, 3)] * rng.choice((0, 0, 0, 1, 5))
+    if seed == 0:
+        left = [x for slot in range(n) for x in sorted(y for y in left if y[0] == slot)]      # whole streams, one behind the other
+    if seed == 1:
+        left = left[::-1]                                                                     # positions fall
+    rows = len(left)
+    assert rows > 300
+    qkv, (cos, sin) = rand((rows, 5 * 128), dev, seed), tables(range(rows), dev)
+    st, pos = i32([s for s, _ in left], dev), i32([p for _, p in left], dev)
+    out = []
+    for step in (rows, 37):
+        kv = (ops.Kv4Arena if bits == 4 else ops.KvArena)(n, 1, kv_heads, lmax, dev)
+        for i in range(0, rows, step):
+            ops.qk_norm_rope_kv_append(qkv[i:i + step], cos[i:i + step], sin[i:i + step], st[i:i + step], pos[i:i + step], kv, 0, heads)
+        out.append(kv.buf)
+    assert torch.equal(*out)
