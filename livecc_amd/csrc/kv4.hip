@@ -675,18 +675,18 @@ static void kv4_combine(const float* ws_o, const float* ws_ml, bf16_t* out, cons
   else kv4_combine_kernel<4><<<dim3(items, n_tiles), dim3(256), 0, st>>>(ws_o, ws_ml, out, tile_q0, tile_nq, tile_rows, n_rows, n_q_heads, nsplit);
 }
 
-// Key splits of a decode step, by its blocks without any (rows x KV heads; a unit holds one) and the 32-key blocks of its longest row.  Measured (us, lengths spread over a quarter):
-//   Up to 32 key blocks: none; 28 / 4 heads, one row of 300 keys 5.0, in eight 6.3, of 1,000 7.7 / 6.8.
+// Key splits of a decode step, by its blocks without any (rows x KV heads; a unit takes one well) and the 32-key blocks of its longest row.  Measured (us, lengths spread over a quarter or fifth):
+//   Up to 32 key blocks: none, one launch.  28 / 4 heads, one row of 300 keys 5.0, in eight 6.3; of 1,000 7.7 / 6.8, which a second launch's issue takes back.
 //   Up to 32 blocks: a block for every unit.  One row of 32,000 keys 16 / 64 splits 16.6 / 10.2, 8 rows of 6,144 4 / 8 / 16 splits 13.7 / 11.1 / 12.0.
 //   Up to 64: as many, from 64 key blocks on: 16 rows of 1,100 keys 1 / 4 splits 7.6 / 8.4, of 2,400 12.8 / 10.3; eight from 192 on: of 6,144 14.4 / 14.6, of 16,000 33.5 / 28.7.
-//   Up to 192: eight, from 96 on.  Their lengths even out, and more waves load at a time: 40 rows of 2,400 keys 1 / 2 / 8 splits 13.6 / 16.5 / 16.6, of 6,144 34.0 / 36.2 / 30.1; 24 rows of 2,400
-//   13.0 / 12.7 / 12.7, of 6,144 26.2 / 20.4 / 18.0; 48 of 16,000 88.6 / 90.6 / 74.9.
-//   More: none.  56 rows of 6,144 keys 1 / 6 splits 41.1 / 40.3, 64 rows 45.2 / 44.9, of 2,400 15.8 / 20.4.
+//   More: eight, from 96 key blocks on, where the blocks leave a fifth of the units or more idle in their last round: 40 rows of 2,400 keys 1 / 2 / 8 splits 13.6 / 16.5 / 16.6, of 6,144
+//   34.0 / 36.2 / 30.1; 24 rows of 2,400 13.0 / 12.7 / 12.7, of 6,144 26.2 / 20.4 / 18.0; 48 of 16,000 88.6 / 90.6 / 74.9; 80 of 6,000 65.4 / 59.7 / 53.7.  Where the round is full, from 320 on:
+//   64 rows of 6,144 keys 1 / 6 splits 45.2 / 44.9, 56 rows 41.1 / 40.3, 128 rows of 6,000 1 / 8 splits 83.8 / 84.1, of 12,000 161.3 / 160.0, with lengths over two thirds 128.8 / 124.9.
 int kv4_decode_splits(const int32_t* n_keys, int n, int n_kv_heads) {
   long most = 1;
   for (int i = 0; i < n; ++i) most = n_keys[i] > most ? n_keys[i] : most;
-  const long keys = (most + 31) / 32, base = (long)(n > 0 ? n : 1) * n_kv_heads, units = (256 + base - 1) / base;
-  if (keys <= 32 || base > 192 || (base > 32 && keys < 64) || (base > 64 && keys < 96)) return 1;
+  const long keys = (most + 31) / 32, base = (long)(n > 0 ? n : 1) * n_kv_heads, units = (256 + base - 1) / base, rounds = (base + 255) / 256;
+  if (keys <= 32 || (base > 32 && keys < 64) || (base > 64 && (keys < 96 || (base * 5 > rounds * 256 * 4 && keys < 320)))) return 1;
   const long k = base > 64 || (base > 32 && keys >= 192) ? 8 : units;
   return (int)std::max(std::min(k, std::min(keys / 4, 64L)), 1L);
 }
