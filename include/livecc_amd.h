@@ -323,8 +323,9 @@ int lcc_sample_topk_topp(const void* logits, int ld, int B, int V, uint32_t* see
  * lmax % 32 == 0); a slot's arena has lcc_kv4_slot_bytes(lay) bytes, 16-byte aligned:
  *   [layer][K codes [head][lmax][64] | V codes [head][lmax / 32][g 4][i 16][t 4][e 8] | K scales [head][lmax][4] | V scales [head][lmax / 32][g 4][t 4][e 8]]
  *   K: byte b of a token = channels 2 b (low half), 2 b + 1;  V: byte (g, i, t, e) = position 8 g + e of the block, channels 32 t + i (low half), 32 t + 16 + i.
- * kv_base: device table of n_slots arenas.  Slots and positions are checked on the device: a row whose slot or position is out of range (-1: a padded
- * row) appends nothing, reads and attends to nothing (zeros).  (slot, position) pairs of one append are distinct. */
+ * kv_base: device table of n_slots arenas.  Slots and positions are checked on the device.  A row whose slot is out of range or whose position is below zero (-1: a padded
+ * row) appends nothing, reads and attends to nothing (zeros).  At a position of lmax or more it appends and reads nothing, too, and attends to all lmax keys.
+ * (slot, position) pairs of one append are distinct. */
 size_t lcc_kv4_slot_bytes(lcc_kv_layout lay);                                   /* 0: invalid layout */
 /* Between the q|k|v projection and the attention, one pass: [RMS norm of every query and key head: bf16(w * bf16(x * r)), r = 1 / sqrt(mean(x^2) + eps) formed
  * in 64 bits and rounded once] + M-RoPE (as lcc_rope_kv_append_bf16) + append.  q_norm / k_norm: bf16 [128], NULL: no norm.  Rows: qkv_bf16

@@ -747,7 +747,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_chunk_kv4_kernel(Kv4Args a, c
   const int nst = (nk + KV4_STAGE - 1) / KV4_STAGE, per = (nst + nsplit - 1) / nsplit, s0 = split * per, s1 = min(nst, s0 + per);
   const int c = wave * 32 + col, r = c / G, h = c - r * G;
   const bool valid = r < nq;
-  const int lim = live ? pos0 + min(r, nq - 1) : -1;                        // last key this column sees
+  const int lim = live ? min(pos0 + min(r, nq - 1), a.lmax - 1) : -1;       // last key this column sees: an arena may end inside a stage, whose other keys are none
 
   u32x4 qf[8];
   const bf16_t* qp = q + ((size_t)(q0 + min(r, nq - 1)) * n_q_heads + hk * G + h) * 128 + hh * 8;

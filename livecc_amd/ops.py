@@ -545,8 +545,8 @@ def kv4_decode_splits(n_keys: Sequence[int], n_kv_heads: int) -> int:
 
 
 def attn_decode4(q: torch.Tensor, kv: Kv4Arena, layer: int, slots: torch.Tensor, kv_len: torch.Tensor, n_q_heads: int, nsplit: int = 0) -> torch.Tensor:
-    """`attn_decode` over the 4-bit cache: row b sees keys 0 .. kv_len[slots[b]] of its slot (none at -1, or for a slot out of range: zeros).  nsplit 0: the split
-    count that suits streams as long as the arena; callers that know the lengths take it from `kv4_decode_splits`."""
+    """`attn_decode` over the 4-bit cache: row b sees keys 0 .. kv_len[slots[b]] of its slot (none at -1, or for a slot out of range: zeros; all that the arena has at a length
+    of lmax or more, whose token's own key the append has dropped).  nsplit 0: the split count that suits streams as long as the arena; callers that know the lengths take it from `kv4_decode_splits`."""
     _kv4(kv)
     if nsplit == 0:
         nsplit = kv4_decode_splits([kv.lmax] * max(1, q.shape[0]), kv.n_kv_heads)

@@ -704,3 +704,37 @@ def test_append_of_runs_of_all_lengths(dev, bits, seed):
             ops.qk_norm_rope_kv_append(qkv[i:i + step], cos[i:i + step], sin[i:i + step], st[i:i + step], pos[i:i + step], kv, 0, heads)
         out.append(kv.buf)
     assert torch.equal(*out)
+
+
+def by_tiles(through, q, kv, tiles, heads, height, nsplit):
+    """Attention of chunks by tiles (slot, first row, rows, first position) below the Python wrapper, which refuses positions behind the arena."""
+    import ctypes
+    from livecc_amd import _lib, torch_ops
+    S, t = q.shape[0], i32([list(c) for c in zip(*tiles)], q.device)
+    if through == "torch":
+        return torch_ops.load().attn_prefill4(q, kv.ptrs, kv.buf, kv.n_layers, kv.n_kv_heads, kv.lmax, 0, t, heads, height, nsplit)
+    out, ws = torch.empty_like(q), torch.empty(S * heads * nsplit * 130, device=q.device)
+    at, n, st = t.data_ptr(), 4 * len(tiles), ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    _lib.check(_lib.load().lcc_attn_prefill_kv4(q.data_ptr(), out.data_ptr(), at, at + n, at + 2 * n, at + 3 * n, kv.ptrs.data_ptr(), kv.buf.shape[0], kv.lay, 0, len(tiles), heads,
+                                                height, nsplit, S, ws.data_ptr(), ws.data_ptr() + S * heads * nsplit * 512, st), "lcc_attn_prefill_kv4")
+    return out
+
+
+@pytest.mark.parametrize("through", ["torch", "ctypes"])
+@pytest.mark.parametrize("columns", [16, 128, 256])
+@pytest.mark.parametrize("nsplit", [1, 2])
+@pytest.mark.parametrize("lmax", [32, 96, 128, 160])
+def test_chunk_rows_behind_the_arena_see_all_of_it(dev, through, columns, nsplit, lmax):
+    """A row at a position of lmax or more sees keys 0 .. lmax - 1, whatever the tile's height, and whether the arena ends inside a stage of 64 keys or with one."""
+    heads, kv_heads, height = 14, 2, columns * 2 // 14
+    kv = filled(dev, rand((2, kv_heads, lmax, 128), dev, 1), rand((2, kv_heads, lmax, 128), dev, 2))
+    runs = [(0, 10, lmax - 6), (1, 3, lmax), (1, 2, lmax + 31), (0, 2, 2 ** 31 - 2)]
+    tiles, at, S = [], [], sum(n for _, n, _ in runs)
+    for slot, n, pos in runs:
+        tiles += [(slot, len(at) + o, min(height, n - o), pos + o) for o in range(0, n, height)]
+        at += [(slot, pos + r) for r in range(n)]
+    q = rand((S, heads * 128), dev, 3)
+    got = by_tiles(through, q, kv, tiles, heads, height, nsplit)
+    for i, (slot, p) in enumerate(at):
+        want, tol = U.attention(q[i:i + 1].cpu().view(1, heads, 128), *values(kv, slot), [min(p, lmax - 1)])
+        U.assert_within(got[i], want[0].flatten(), tol[0].flatten(), f"row {i}, position {p} of {lmax}")
