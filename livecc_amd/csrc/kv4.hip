@@ -455,8 +455,9 @@ int kv4_read(const Kv4Args& a, const int32_t* tok_stream, const int32_t* tok_pos
 // 32,768 keys (64 / 8 heads, 64 splits) 10 us for 36 MB, of which some 4 are the launch and the first trip.
 // The same kernel takes tiles of a few rows of a chunk (CHUNK): its columns are then (row, head) pairs.
 // ------------------------------------------------------------------------------------------------------------------------------
-// The maximum that a softmax subtracts moves when a score passes it by more than 2^KV4_SLACK, not at every new one: sums and products scale alike, probabilities stay below
-// 2^8, and bf16's and fp32's relative steps are the same there.  Where it does not move, eight (chunks: 64) multiplications of O a block fall away.
+// What a softmax subtracts, m, lies KV4_SLACK (in powers of two) above the highest score at which it last moved, and moves when a score passes it, not at every new maximum: sums and
+// products scale alike, and bf16's and fp32's relative steps are the same at 2^-8.  Where it does not move, eight (chunks: 64) multiplications of O a block fall away.  Weights are never
+// above one, so that a product p V leaves fp32's range only where the sum of the values does.
 constexpr float KV4_SLACK = 8.f;
 struct Kv4Tile { u32x4 k[2], v[2], s[2]; unsigned ks[2]; };       // what a wave loads of a 32-key block: codes of two key tiles, of V, V's scales, K's
 struct Kv4Head { const uint8_t *kc, *vc, *ks, *vs; };              // a head's regions, wave-uniform: a lane's part of the addresses is 32 bits that never change
@@ -557,8 +558,8 @@ __global__ __launch_bounds__(NW * 64, 4) void attn_rows_kv4_kernel(Kv4Args a, Kv
       float top = __builtin_fmaxf(__builtin_fmaxf(__builtin_fmaxf(sc[0][0], sc[0][1]), __builtin_fmaxf(sc[0][2], sc[0][3])),
                                   __builtin_fmaxf(__builtin_fmaxf(sc[1][0], sc[1][1]), __builtin_fmaxf(sc[1][2], sc[1][3])));
       top = xor32_max(xor16_max(top)) * scale_log2e;
-      if (__any(top > m + KV4_SLACK)) {
-        const float mn = __builtin_fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+      if (__any(top > m)) {
+        const float mn = top > m ? top + KV4_SLACK : m, f = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
         l *= f;
 #pragma unroll
         for (int t = 0; t < 8; ++t) o[t] *= f;
@@ -908,7 +909,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_chunk_kv4_kernel(Kv4Args a, c
           for (int z = 1; z < 16; ++z) tt = __builtin_fmaxf(tt, sc[i][z]);
         } else if constexpr (i == 2) {
           const float top = xor32_max(__builtin_fmaxf(t0, t1)) * scale_log2e;
-          const float mn = top > m + KV4_SLACK ? top : m;
+          const float mn = top > m ? top + KV4_SLACK : m;
           mu = mn == -INFINITY ? 0.f : mn;
           f = __builtin_amdgcn_exp2f(m - mu);
           m = mn;

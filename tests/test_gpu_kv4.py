@@ -738,3 +738,30 @@ def test_chunk_rows_behind_the_arena_see_all_of_it(dev, through, columns, nsplit
     for i, (slot, p) in enumerate(at):
         want, tol = U.attention(q[i:i + 1].cpu().view(1, heads, 128), *values(kv, slot), [min(p, lmax - 1)])
         U.assert_within(got[i], want[0].flatten(), tol[0].flatten(), f"row {i}, position {p} of {lmax}")
+
+
+def attend(q, kv, heads, nsplit, columns):
+    """one row at the arena's last position: a decode step (columns 0), or a chunk by tiles of so many columns"""
+    from livecc_amd import ops
+    if columns == 0:
+        return ops.attn_decode4(q, kv, 0, i32([0], q.device), i32([kv.lmax - 1], q.device), heads, nsplit)
+    return ops.attn_prefill4(q, kv, 0, ops.kv4_prefill_plan([(0, 1, kv.lmax - 1)], heads, kv.n_kv_heads, q.device, nsplit, columns * kv.n_kv_heads // heads), heads)
+
+
+@pytest.mark.parametrize("columns", [0, 16, 128, 256])
+@pytest.mark.parametrize("nsplit", [1, 2])
+@pytest.mark.parametrize("size", [120, -120])
+def test_large_and_small_values_under_a_rising_maximum(dev, columns, nsplit, size):
+    """Values of 6 * 2^size and keys whose weight is 2^6.1 times that of the keys of the blocks before: every weighted mean is the value itself.  A weight above one would take the large values'
+    products out of fp32's range, weights of 2^-14 take the small ones' below its normal range.  Tolerance: half a step of bf16 for the probabilities, as many for the result, 2^-16 for the
+    sums (a product of 2^-131 is held to 2^-149)."""
+    heads, kv_heads, L = 14, 2, 320
+    k, v = torch.zeros(1, kv_heads, L, 128, dtype=torch.bfloat16, device=dev), torch.full((1, kv_heads, L, 128), 6 * 2.0 ** size, dtype=torch.bfloat16, device=dev)
+    v[..., 1::2] *= -1
+    k[:, :, (130, 258, 290), 7] = 48.0
+    kv = filled(dev, k, v)
+    q = torch.zeros(1, heads, 128, dtype=torch.bfloat16, device=dev)
+    q[..., 7] = 1.0
+    want = v[0, :, 0].double().cpu().repeat_interleave(heads // kv_heads, 0).flatten()[None] * 2.0 ** -size
+    got = attend(q.flatten(1), kv, heads, nsplit, columns).double() * 2.0 ** -size
+    U.assert_within(got, want, want.abs() * (2.0 ** -7 + 2.0 ** -16))
