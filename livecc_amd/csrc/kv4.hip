@@ -455,10 +455,15 @@ int kv4_read(const Kv4Args& a, const int32_t* tok_stream, const int32_t* tok_pos
 // 32,768 keys (64 / 8 heads, 64 splits) 10 us for 36 MB, of which some 4 are the launch and the first trip.
 // The same kernel takes tiles of a few rows of a chunk (CHUNK): its columns are then (row, head) pairs.
 // ------------------------------------------------------------------------------------------------------------------------------
-// What a softmax subtracts, m, lies KV4_SLACK (in powers of two) above the highest score at which it last moved, and moves when a score passes it, not at every new maximum: sums and
+// Scores are sums of products q k; a weight is 2^(KV4_SCALE (score - m)), the difference formed before it is scaled: m scaled by itself is off by half a step, which is more than 2^7 powers of
+// two from scores of 2^35 on.  What a softmax subtracts, m, lies KV4_SLACK (8 powers of two) above the highest score at which it last moved, and moves when a score passes it, not at every new maximum: sums and
 // products scale alike, and bf16's and fp32's relative steps are the same at 2^-8.  Where it does not move, eight (chunks: 64) multiplications of O a block fall away.  Weights are never
 // above one, so that a product p V leaves fp32's range only where the sum of the values does.
-constexpr float KV4_SLACK = 8.f;
+constexpr float KV4_SCALE = 1.4426950408889634 / 11.313708498984761, KV4_SLACK = 8.f / KV4_SCALE;       // log2(e) / sqrt(128)
+// Weights of keys are formed from KV4_SCALE score - (KV4_SCALE m) in one operation where |KV4_SCALE m| is at most this: its rounding is then 2^-13 powers of two at most, a thirtieth of the weight's to
+// bf16.  Beyond, their scores become differences first, a wave at a time (always: eight chunks of ~340 rows 242 -> 251 us, 64 rows of 2,200 to 6,000 keys 32.3 -> 32.6).
+constexpr float KV4_FUSED = 4096.f;
+LCC_DEVICE float kv4_weight(float score, float m) { return __builtin_amdgcn_exp2f((score - m) * KV4_SCALE); }
 struct Kv4Tile { u32x4 k[2], v[2], s[2]; unsigned ks[2]; };       // what a wave loads of a 32-key block: codes of two key tiles, of V, V's scales, K's
 struct Kv4Head { const uint8_t *kc, *vc, *ks, *vs; };              // a head's regions, wave-uniform: a lane's part of the addresses is 32 bits that never change
 LCC_DEVICE void kv4_load_k(Kv4Tile& t, const Kv4Head& h, int blk, unsigned key, unsigned g) {
@@ -480,7 +485,7 @@ struct Kv4Rows { const int32_t* slot; const int32_t* kv_len; const int32_t* q0; 
 
 template <int NW, bool CHUNK>
 __global__ __launch_bounds__(NW * 64, 4) void attn_rows_kv4_kernel(Kv4Args a, Kv4Rows rows, const bf16_t* __restrict__ q, int n_q_heads, int nsplit, float* __restrict__ ws_o,
-                                                                   float* __restrict__ ws_ml, bf16_t* __restrict__ out, float scale_log2e) {
+                                                                   float* __restrict__ ws_ml, bf16_t* __restrict__ out) {
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   float (*mo)[16][132] = reinterpret_cast<float (*)[16][132]>(lds);
   __shared__ float mm[NW][16], ml[NW][16];
@@ -498,7 +503,7 @@ __global__ __launch_bounds__(NW * 64, 4) void attn_rows_kv4_kernel(Kv4Args a, Kv
   f32x4 o[8];
 #pragma unroll
   for (int t = 0; t < 8; ++t) o[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.f;                                             // m in units of log2
+  float m = -INFINITY, l = 0.f;
   int blk = b0 + wave;
   if (blk < b1) {
     const Kv4Layout lay{a.n_kv_heads, a.lmax};
@@ -557,18 +562,19 @@ __global__ __launch_bounds__(NW * 64, 4) void attn_rows_kv4_kernel(Kv4Args a, Kv
       }
       float top = __builtin_fmaxf(__builtin_fmaxf(__builtin_fmaxf(sc[0][0], sc[0][1]), __builtin_fmaxf(sc[0][2], sc[0][3])),
                                   __builtin_fmaxf(__builtin_fmaxf(sc[1][0], sc[1][1]), __builtin_fmaxf(sc[1][2], sc[1][3])));
-      top = xor32_max(xor16_max(top)) * scale_log2e;
+      top = xor32_max(xor16_max(top));
       if (__any(top > m)) {
-        const float mn = top > m ? top + KV4_SLACK : m, f = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+        const float mn = top > m ? top + KV4_SLACK : m, f = kv4_weight(m, mn == -INFINITY ? 0.f : mn);
         l *= f;
 #pragma unroll
         for (int t = 0; t < 8; ++t) o[t] *= f;
         m = mn;
       }
       const float mu = m == -INFINITY ? 0.f : m;                            // a column that has seen no key, or scores of -inf alone
-      float p[8];
+      float p[8], ms = mu * KV4_SCALE;
+      if (__any(__builtin_fabsf(ms) > KV4_FUSED)) { sc[0] -= mu; sc[1] -= mu; ms = 0.f; }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) { p[e] = __builtin_amdgcn_exp2f(fmaf(sc[e >> 2][e & 3], scale_log2e, -mu)); l += p[e]; }
+      for (int e = 0; e < 8; ++e) { p[e] = __builtin_amdgcn_exp2f(fmaf(sc[e >> 2][e & 3], KV4_SCALE, -ms)); l += p[e]; }
       // The products take probabilities in bf16, as the bf16 cache's attention does (l sums them unrounded):
       // each off by half a step at most, 2^-8 of itself, and so the result by 2^-8 of the weighted mean of |V|.
       // A converted byte is a pair (channel i, channel 16 + i) of one key, two slots of the operand: against (p, 0) it is channel i's product, against (0, p) the other's.
@@ -608,7 +614,7 @@ __global__ __launch_bounds__(NW * 64, 4) void attn_rows_kv4_kernel(Kv4Args a, Kv
     f32x4 acc = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
-      const float f = __builtin_amdgcn_exp2f(mm[w][h] - mu);
+      const float f = kv4_weight(mm[w][h], mu);
       L += f * ml[w][h];
       acc += f * *reinterpret_cast<const f32x4*>(&mo[w][h][c]);
     }
@@ -624,7 +630,7 @@ __global__ __launch_bounds__(NW * 64, 4) void attn_rows_kv4_kernel(Kv4Args a, Kv
   }
 }
 
-// Joins the key splits of a (row, head): sums weighted by 2^(m - max), one rounding.  A half-wave reads a split's 128 channels at a time; W waves share a (row, head).
+// Joins the key splits of a (row, head): sums weighted by their m's distance from the highest, one rounding.  A half-wave reads a split's 128 channels at a time; W waves share a (row, head).
 // blockIdx.y: a tile, or (tiles null) a row.  All loads of a (row, head) are in flight before the first weight is known; a trip's time otherwise: 64 splits of 64 heads 3.6 us,
 // of 17 rows x 28 4.3 us (15.8 MB), five of 386 rows 7.6 us (28 MB, 3.7 TB/s).  In one wave (W = 1) to 8 splits, in four beyond: those have more to load than registers.
 template <int W>
@@ -647,7 +653,7 @@ __global__ __launch_bounds__(256) void kv4_combine_kernel(const float* __restric
     v[i] = s < nsplit ? *reinterpret_cast<const f32x4*>(o + (size_t)s * 128) : (f32x4){0.f, 0.f, 0.f, 0.f};
   }
   const float m = lane < nsplit ? ml[lane * 2] : -INFINITY, l = lane < nsplit ? ml[lane * 2 + 1] : 0.f;
-  const float M = wave_max(m), w = __builtin_amdgcn_exp2f(m - (M == -INFINITY ? 0.f : M));
+  const float M = wave_max(m), w = kv4_weight(m, M == -INFINITY ? 0.f : M);
   const float L = wave_sum(w * l);
   f32x4 acc = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -699,9 +705,8 @@ static void attn_rows_launch(const Kv4Args& a, const Kv4Rows& rows, int n, const
   constexpr int part = 16 * 132 * 4;                                        // LDS of a wave's result
   if (once.first()) (void)hipFuncSetAttribute((const void*)attn_rows_kv4_kernel<8, CHUNK>, hipFuncAttributeMaxDynamicSharedMemorySize, 8 * part);
   const dim3 grid(nsplit, a.n_kv_heads, n);
-  const float scale = 1.4426950408889634f / sqrtf(128.f);
-  if (nsplit == 1) attn_rows_kv4_kernel<8, CHUNK><<<grid, dim3(512), 8 * part, st>>>(a, rows, q, n_q_heads, nsplit, ws_o, ws_ml, out, scale);
-  else attn_rows_kv4_kernel<4, CHUNK><<<grid, dim3(256), 4 * part, st>>>(a, rows, q, n_q_heads, nsplit, ws_o, ws_ml, out, scale);
+  if (nsplit == 1) attn_rows_kv4_kernel<8, CHUNK><<<grid, dim3(512), 8 * part, st>>>(a, rows, q, n_q_heads, nsplit, ws_o, ws_ml, out);
+  else attn_rows_kv4_kernel<4, CHUNK><<<grid, dim3(256), 4 * part, st>>>(a, rows, q, n_q_heads, nsplit, ws_o, ws_ml, out);
 }
 
 int attn_decode_kv4(const Kv4Args& a, const bf16_t* q, const int32_t* slots, const int32_t* kv_len, int rows, int n_q_heads, int nsplit, float* ws_o, float* ws_ml,
@@ -734,7 +739,7 @@ template <int NW>
 __global__ __launch_bounds__(NW * 64, 2) void attn_chunk_kv4_kernel(Kv4Args a, const bf16_t* __restrict__ q, bf16_t* __restrict__ out, const int32_t* __restrict__ tile_stream,
                                                                       const int32_t* __restrict__ tile_q0, const int32_t* __restrict__ tile_nq,
                                                                       const int32_t* __restrict__ tile_pos0, int n_q_heads, int tile_rows, int nsplit, int n_rows,
-                                                                      float* __restrict__ ws_o, float* __restrict__ ws_ml, float scale_log2e) {
+                                                                      float* __restrict__ ws_o, float* __restrict__ ws_ml) {
   constexpr int U = 8 / NW;                                                 // units of 8 bytes of K and of V that a thread stages
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   __shared__ unsigned long long bad[4][4];                                  // keys of a stage, by group, whose V is NaN (stages with masked scores)
@@ -896,7 +901,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_chunk_kv4_kernel(Kv4Args a, c
       // 32 products, their operands read four ahead, and the vector work dealt out between them
       u32x4 fr[5], pn[4];
       unsigned cv[8];
-      float t0 = 0.f, t1 = 0.f, mu = 0.f, f = 1.f;
+      float t0 = 0.f, t1 = 0.f, mu = 0.f, ms = 0.f, f = 1.f;
       unrolled<4>([&](auto I) { fr[decltype(I)::value] = operand(I, st); });
       unrolled<32>([&](auto I) {
         constexpr int i = decltype(I)::value;
@@ -908,15 +913,21 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_chunk_kv4_kernel(Kv4Args a, c
 #pragma unroll
           for (int z = 1; z < 16; ++z) tt = __builtin_fmaxf(tt, sc[i][z]);
         } else if constexpr (i == 2) {
-          const float top = xor32_max(__builtin_fmaxf(t0, t1)) * scale_log2e;
+          const float top = xor32_max(__builtin_fmaxf(t0, t1));
           const float mn = top > m ? top + KV4_SLACK : m;
           mu = mn == -INFINITY ? 0.f : mn;
-          f = __builtin_amdgcn_exp2f(m - mu);
+          f = kv4_weight(m, mu);
           m = mn;
           l *= f;
+          ms = mu * KV4_SCALE;
+          if (__any(__builtin_fabsf(ms) > KV4_FUSED)) {
+#pragma unroll
+            for (int z = 0; z < 32; ++z) sc[z >> 4][z & 15] -= mu;
+            ms = 0.f;
+          }
         } else if constexpr (i < 19) {                                      // two probabilities: the first tile's before its scores are overwritten, the second's too
           constexpr int k = i - 3;
-          const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[k >> 3][(2 * k) & 15], scale_log2e, -mu)), p1 = __builtin_amdgcn_exp2f(fmaf(sc[k >> 3][(2 * k + 1) & 15], scale_log2e, -mu));
+          const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[k >> 3][(2 * k) & 15], KV4_SCALE, -ms)), p1 = __builtin_amdgcn_exp2f(fmaf(sc[k >> 3][(2 * k + 1) & 15], KV4_SCALE, -ms));
           l += p0 + p1;
           pn[k >> 2][k & 3] = pack2(p0, p1);
         } else if constexpr (i < 19 + 2 * U) {                              // V a unit at a time: converted, put
@@ -1037,13 +1048,12 @@ int attn_prefill_kv4(const Kv4Args& a, const bf16_t* q, bf16_t* out, const int32
     (void)hipFuncSetAttribute((const void*)attn_chunk_kv4_kernel<4>, hipFuncAttributeMaxDynamicSharedMemorySize, KV4_LDS);
   }
   const dim3 grid(a.n_kv_heads, n_tiles, nsplit);
-  const float scale = 1.4426950408889634f / sqrtf(128.f);
   if (tile_rows * (n_q_heads / a.n_kv_heads) <= 16)
     attn_rows_launch<true>(a, Kv4Rows{tile_stream, nullptr, tile_q0, tile_nq, tile_pos0, tile_rows, n_rows}, n_tiles, q, n_q_heads, nsplit, ws_o, ws_ml, out, st);
   else if (tile_rows * (n_q_heads / a.n_kv_heads) > 128)
-    attn_chunk_kv4_kernel<8><<<grid, dim3(512), KV4_LDS, st>>>(a, q, out, tile_stream, tile_q0, tile_nq, tile_pos0, n_q_heads, tile_rows, nsplit, n_rows, ws_o, ws_ml, scale);
+    attn_chunk_kv4_kernel<8><<<grid, dim3(512), KV4_LDS, st>>>(a, q, out, tile_stream, tile_q0, tile_nq, tile_pos0, n_q_heads, tile_rows, nsplit, n_rows, ws_o, ws_ml);
   else
-    attn_chunk_kv4_kernel<4><<<grid, dim3(256), KV4_LDS, st>>>(a, q, out, tile_stream, tile_q0, tile_nq, tile_pos0, n_q_heads, tile_rows, nsplit, n_rows, ws_o, ws_ml, scale);
+    attn_chunk_kv4_kernel<4><<<grid, dim3(256), KV4_LDS, st>>>(a, q, out, tile_stream, tile_q0, tile_nq, tile_pos0, n_q_heads, tile_rows, nsplit, n_rows, ws_o, ws_ml);
   if (nsplit > 1) kv4_combine(ws_o, ws_ml, out, tile_q0, tile_nq, n_tiles, tile_rows, n_rows, n_q_heads, nsplit, st);
   return 0;
 }

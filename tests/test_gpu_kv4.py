@@ -765,3 +765,37 @@ def test_large_and_small_values_under_a_rising_maximum(dev, columns, nsplit, siz
     want = v[0, :, 0].double().cpu().repeat_interleave(heads // kv_heads, 0).flatten()[None] * 2.0 ** -size
     got = attend(q.flatten(1), kv, heads, nsplit, columns).double() * 2.0 ** -size
     U.assert_within(got, want, want.abs() * (2.0 ** -7 + 2.0 ** -16))
+
+
+@pytest.mark.parametrize("columns", [0, 16, 128, 256])
+@pytest.mark.parametrize("nsplit", [1, 2, 5])
+@pytest.mark.parametrize("order", ["rising", "falling"])
+def test_scores_of_any_size(dev, columns, nsplit, order):
+    """Scores of 2^30 to 2^113, of more bits than fp32 holds once they are scaled, whose neighbours lie so far apart that the keys of the highest share all of the weight: their mean.
+    Tolerance: half a step of bf16 for the result, none for the weights (all one), 2^-16 for the sums."""
+    heads, kv_heads, L = 14, 2, 320
+    k, v = torch.zeros(1, kv_heads, L, 128, dtype=torch.bfloat16, device=dev), rand((1, kv_heads, L, 128), dev, 2)
+    steps = torch.tensor([1.0, 1.5, 2.0, 3.0, 4.0], device=dev).repeat_interleave(64)
+    k[..., 7] = steps if order == "rising" else steps.flip(0)
+    k[..., 45, 7] = 4.0
+    kv = filled(dev, k, v)
+    size = [30, 31, 32, 33, 34, 35, 36, 37, 38, 40, 47, 60, 77, 110]
+    for sign in (1, -1):
+        top = (k[0, 0, :, 7] == (4.0 if sign > 0 else 1.0)).cpu()
+        vv = values(kv, 0)[1][:, top].repeat_interleave(heads // kv_heads, 0)
+        want, tol = vv.mean(1), 2.0 ** -8 * vv.mean(1).abs() + 2.0 ** -16 * vv.abs().mean(1)
+        q = torch.zeros(1, heads, 128, dtype=torch.bfloat16, device=dev)
+        q[0, :, 7] = sign * torch.pow(2.0, torch.tensor(size, device=dev)) * (1 + (2 * torch.arange(heads, device=dev) * 9 % 64 + 1) / 128)
+        U.assert_within(attend(q.flatten(1), kv, heads, nsplit, columns), want.flatten()[None], tol.flatten()[None], f"sign {sign}")
+
+
+@pytest.mark.parametrize("columns", [0, 16, 128, 256])
+@pytest.mark.parametrize("nsplit", [1, 3])
+def test_heads_of_very_different_scores(dev, columns, nsplit):
+    """queries of 1 to 4,096 times the usual size in one call: scores of a few units beside ones of several thousand, in the same wave"""
+    heads, kv_heads, L = 14, 2, 288
+    kv = filled(dev, rand((1, kv_heads, L, 128), dev, 1), rand((1, kv_heads, L, 128), dev, 2))
+    size = torch.pow(2.0, (torch.arange(heads) * 5 % 13).double())
+    q = (rand((1, heads, 128), "cpu", 3) * size[None, :, None].to(torch.bfloat16)).to(dev)
+    want, tol = U.attention(q.cpu(), *values(kv, 0), [L - 1])
+    U.assert_within(attend(q.flatten(1), kv, heads, nsplit, columns), want.flatten(1), tol.flatten(1))
