@@ -487,6 +487,7 @@ def qk_norm_rope_kv_append(qkv: Optional[torch.Tensor], cos, sin, tok_stream, to
                          (q_norm, (128,), "q_norm"), (k_norm, (128,), "k_norm")):
         if a is not None:
             _shape(a, shape, nm)
+    _no_graph(qkv=qkv, partial=partial, bias=bias, q_norm=q_norm, k_norm=k_norm, cos=cos, sin=sin)
     q = torch.empty(S, n_q_heads * 128, dtype=torch.bfloat16, device=cos.device)
     if S == 0:
         return q
@@ -504,6 +505,13 @@ def _same_device(like: torch.Tensor, **others) -> None:
     for name, t in others.items():
         if t is not None and t.device != like.device:
             raise ValueError(f"{name}: on {t.device}, the rows are on {like.device}")
+
+
+def _no_graph(**tensors) -> None:
+    if torch.is_grad_enabled():                    # the registered ops' own rule: a parameter keeps requires_grad where no graph is recorded
+        for name, t in tensors.items():
+            if t is not None and t.requires_grad:
+                raise _lib.LccError(f"{name}: livecc_amd ops are inference ops (no autograd formula): call under torch.no_grad()")
 
 
 def _shape(t: torch.Tensor, shape, name: str) -> None:
@@ -554,7 +562,7 @@ def attn_decode4(q: torch.Tensor, kv: Kv4Arena, layer: int, slots: torch.Tensor,
         t = _T.op("attn_decode4")
         if t is not None:
             return t(q, kv.ptrs, kv.buf, kv.n_layers, kv.n_kv_heads, kv.lmax, layer, slots, kv_len, n_q_heads, nsplit)
-    _chk(q, torch.bfloat16, "q"), _chk(slots, torch.int32, "slots"), _chk(kv_len, torch.int32, "kv_len")
+    _chk(q, torch.bfloat16, "q"), _chk(slots, torch.int32, "slots"), _chk(kv_len, torch.int32, "kv_len"), _no_graph(q=q)
     B, n_slots = q.shape[0], kv.buf.shape[0]
     _same_device(q, slots=slots, kv_len=kv_len, kv=kv.buf), _shape(q, (B, n_q_heads * 128), "q"), _shape(slots, (B,), "slots")
     if kv_len.numel() < n_slots:
@@ -611,7 +619,7 @@ def attn_prefill4(q: torch.Tensor, kv: Kv4Arena, layer: int, plan, n_q_heads: in
         t = _T.op("attn_prefill4")
         if t is not None:
             return t(q, kv.ptrs, kv.buf, kv.n_layers, kv.n_kv_heads, kv.lmax, layer, plan.tiles, n_q_heads, plan.tile_rows, plan.nsplit)
-    _chk(q, torch.bfloat16, "q"), _chk(plan.tiles, torch.int32, "plan")
+    _chk(q, torch.bfloat16, "q"), _chk(plan.tiles, torch.int32, "plan"), _no_graph(q=q)
     S, nt = q.shape[0], plan.tiles.shape[1]
     _same_device(q, plan=plan.tiles, kv=kv.buf), _shape(q, (S, n_q_heads * 128), "q")
     out = torch.empty_like(q)

@@ -799,3 +799,30 @@ def test_heads_of_very_different_scores(dev, columns, nsplit):
     q = (rand((1, heads, 128), "cpu", 3) * size[None, :, None].to(torch.bfloat16)).to(dev)
     want, tol = U.attention(q.cpu(), *values(kv, 0), [L - 1])
     U.assert_within(attend(q.flatten(1), kv, heads, nsplit, columns), want.flatten(1), tol.flatten(1))
+
+
+@pytest.mark.parametrize("through", ["torch", "ctypes"])
+def test_no_route_loses_a_gradient(dev, through, monkeypatch):
+    """Whichever input would record a gradient is refused, through the registered ops and through the C-ABI binding; under no_grad all of them may be parameters."""
+    from livecc_amd import ops, torch_ops
+    if through == "ctypes":
+        monkeypatch.setattr(torch_ops, "op", lambda name: None)
+    heads, kv_heads, at = 4, 2, i32([0], dev)
+    kv = ops.Kv4Arena(1, 1, kv_heads, 64, dev)
+    cos, sin = tables([0], dev)
+    rows = dict(qkv=rand((1, 8 * 128), dev, 1), q_norm=rand((128,), dev, 2), k_norm=rand((128,), dev, 3), cos=cos, sin=sin)
+    slabs = dict(qkv=None, partial=rand((2, 1, 8 * 128), dev, 4).float(), bias=rand((8 * 128,), dev, 5), cos=cos, sin=sin)
+
+    def append(qkv, cos, sin, **kw):
+        return ops.qk_norm_rope_kv_append(qkv, cos, sin, at, at, kv, 0, heads, **kw)
+    calls = [(append, a, name) for a in (rows, slabs) for name, t in a.items() if t is not None]
+    calls += [(lambda q: ops.attn_decode4(q, kv, 0, at, at, heads), dict(q=rand((1, heads * 128), dev, 6)), "q"),
+              (lambda q: ops.attn_prefill4(q, kv, 0, [(0, 1, 0)], heads), dict(q=rand((1, heads * 128), dev, 6)), "q")]
+    for call, args, name in calls:
+        args = dict(args, **{name: args[name].clone().requires_grad_()})
+        before = kv.buf.clone()
+        with pytest.raises(RuntimeError, match="no_grad"):
+            call(**args)
+        assert torch.equal(kv.buf, before), name
+        with torch.no_grad():
+            assert not call(**args).requires_grad
