@@ -501,7 +501,7 @@ static void vit32_launch_t(const bf16_t* qkv, const bf16_t* vt, bf16_t* out, con
                            const int32_t* seg_len, const int32_t* seg_blk_start, int n_groups, int heads, int total_blocks, float scale_log2e, hipStream_t st) {
   constexpr size_t lds = Attn32Image<80, 80>::BYTES;
   static DeviceOnce once;   // per instantiation
-  if (once.first()) (void)hipFuncSetAttribute((const void*)attn_vit32_kernel<NWAVE>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  if (auto turn = once.first()) (void)hipFuncSetAttribute((const void*)attn_vit32_kernel<NWAVE>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
   const long nvb = (long)n_groups * heads;
   const int cap = get_grid_cap();
   static const int xcd = [] { const char* v = getenv("LCC_ATTN32_XCD"); return v ? atoi(v) : 1; }();      // A/B: 0 = virtual block = physical block
@@ -579,7 +579,7 @@ int attn_prefill32_launch(const bf16_t* q, bf16_t* out, const int32_t* tile_stre
   if (G < 1 || G > 8 || lay.head_dim != 128) return LCC_ERR_SHAPE;
   constexpr size_t lds = Attn32Image<128, 128>::BYTES;
   static DeviceOnce once;
-  if (once.first()) {
+  if (auto turn = once.first()) {
     (void)hipFuncSetAttribute((const void*)attn_gqa32_kernel<8>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     (void)hipFuncSetAttribute((const void*)attn_gqa32_kernel<4>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
   }
@@ -680,7 +680,7 @@ template <int DK, int DV, bool SLOTS>
 static void mha32_go(const MhaArgs& a, hipStream_t st) {
   constexpr size_t lds = Attn32Image<DK, DV>::BYTES;
   static DeviceOnce once;   // per instantiation
-  if (once.first()) (void)hipFuncSetAttribute((const void*)attn_mha32_kernel<DK, DV, SLOTS>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  if (auto turn = once.first()) (void)hipFuncSetAttribute((const void*)attn_mha32_kernel<DK, DV, SLOTS>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
   const long n_items = (long)a.n_groups * a.heads;
   attn_mha32_kernel<DK, DV, SLOTS><<<dim3((unsigned)((n_items + 7) / 8 * 8)), dim3(512), lds, st>>>(a);
 }

@@ -613,7 +613,7 @@ bool dgemv_rows8_ok(int M, int N, int K, const float* wscale) { return g_resid_w
 template <int EPI, int NW, int XP>
 static void launch_rows8_as(const DgArgs& a, hipStream_t st) {
   static DeviceOnce attr;
-  if (attr.first()) (void)hipFuncSetAttribute((const void*)dgemv_rows8_kernel<EPI, NW, XP>, hipFuncAttributeMaxDynamicSharedMemorySize, ROWS8_LDS);
+  if (auto turn = attr.first()) (void)hipFuncSetAttribute((const void*)dgemv_rows8_kernel<EPI, NW, XP>, hipFuncAttributeMaxDynamicSharedMemorySize, ROWS8_LDS);
   dgemv_rows8_kernel<EPI, NW, XP><<<dim3(a.N / 8), dim3(NW * 64), (size_t)a.M * (a.K + X_PAD) * 2, st>>>(a);
 }
 template <int EPI>

@@ -786,7 +786,7 @@ static void launch_resize_tile(const uint8_t* src, int layout, int T, int Hin, i
                                int rows_cap, int seg_dw, size_t lds, hipStream_t st) {
   const dim3 grid((unsigned)((size_t)T * ((Hout + TH - 1) / TH) * ((Wout + RS_COLS - 1) / RS_COLS)));
   static DeviceOnce attr_set;   // per instantiation
-  if (attr_set.first()) {
+  if (auto turn = attr_set.first()) {
     (void)hipFuncSetAttribute((const void*)resize_aa_tile_kernel<K, false>, hipFuncAttributeMaxDynamicSharedMemorySize, RS_LDS_MAX);
     (void)hipFuncSetAttribute((const void*)resize_aa_tile_kernel<K, true>, hipFuncAttributeMaxDynamicSharedMemorySize, RS_LDS_MAX);
   }

@@ -1804,7 +1804,7 @@ static void launch_mid_w(const GemmArgs& a, hipStream_t st) {
   const int tiles_m = (a.M + 127) / 128, tiles_n = (a.N + 127) / 128, nkt = a.K / 64, S = (EPI == EPI_PARTIAL) ? a.nsplit : 1;
   constexpr size_t lds = (size_t)MID_STAGES * (16384 + (W8 ? 8192 : 16384));
   static DeviceOnce attr_set;   // per instantiation
-  if (attr_set.first()) (void)hipFuncSetAttribute((const void*)gemm_mid_kernel<EPI, W8>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  if (auto turn = attr_set.first()) (void)hipFuncSetAttribute((const void*)gemm_mid_kernel<EPI, W8>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
   gemm_mid_kernel<EPI, W8><<<dim3(capped_grid((long)tiles_m * tiles_n), S), dim3(512), lds, st>>>(
       a.A, a.lda, a.W, a.bias, a.residual, a.ldr, a.C, a.ldc, a.M, a.N, a.K, tiles_m, tiles_n, a.partial, (nkt + S - 1) / S, a.wscale, raster_for(tiles_m), a.vq);
 }
@@ -1827,7 +1827,7 @@ static void launch_strip_w(const GemmArgs& a, hipStream_t st) {
   const int extra = tiles * S < 256 ? strip_fetch_blocks((int)tiles, a.N, S, nkt, W8, &fetch) : 0;
   constexpr size_t lds = (size_t)STRIP_STAGES * 8192;
   static DeviceOnce attr_set;   // per instantiation
-  if (attr_set.first()) (void)hipFuncSetAttribute((const void*)gemm_strip_kernel<EPI, W8>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  if (auto turn = attr_set.first()) (void)hipFuncSetAttribute((const void*)gemm_strip_kernel<EPI, W8>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
   gemm_strip_kernel<EPI, W8><<<dim3(capped_grid(tiles) + extra, S), dim3(256), lds, st>>>(
       a.A, a.lda, a.W, a.bias, a.residual, a.ldr, a.C, a.ldc, a.M, a.N, a.K, tiles_m, tiles_n, a.partial, nkt, a.wscale, raster_for(tiles_m), fetch, a.vq);
 }
@@ -1843,7 +1843,7 @@ static void launch_tiled(const GemmArgs& a, hipStream_t st) {
   if (g_gemm_variant == 1 || ((g_gemm_variant == 2 || g_gemm_variant == 7) && BM == 64)) {   // 7: auto without the 8-wave kernel
     constexpr size_t lds = (size_t)3 * ((BM / 16) * 2 + 16) * 1024;   // 96 KB (BM 128) / 72 KB (BM 64)
     static DeviceOnce attr_set;   // per instantiation
-    if (attr_set.first()) {
+    if (auto turn = attr_set.first()) {
       (void)hipFuncSetAttribute((const void*)gemm_glds_kernel<BM, EPI>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     }
     gemm_glds_kernel<BM, EPI><<<dim3(capped_grid((long)tiles_m * tiles_n), S), dim3(256), lds, st>>>(
@@ -1869,7 +1869,7 @@ static void launch_big_s(const GemmArgs& a, hipStream_t st) {
   // bf16: 128 KB (BM 256, 2 stages) / 144 KB (BM 128, 3 stages); fp8 W: 144 KB (BM 256) / 96 KB (BM 128), 3 stages
   constexpr size_t lds = (size_t)((BM >= 192 && !W8) ? 2 : 3) * (BM * 8 + (W8 ? 1024 : 2048)) * 16;
   static DeviceOnce attr_set;   // per instantiation
-  if (attr_set.first()) {
+  if (auto turn = attr_set.first()) {
     (void)hipFuncSetAttribute((const void*)gemm_big_kernel<BM, EPI, SCHED, W8>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
   }
   gemm_big_kernel<BM, EPI, SCHED, W8><<<dim3(capped_grid((long)tiles_m * tiles_n), S), dim3(512), lds, st>>>(
@@ -1886,7 +1886,7 @@ static void launch_walk(const GemmArgs& a, hipStream_t st) {
   const int nkt = a.K / 64, S = (EPI == EPI_PARTIAL) ? a.nsplit : 1;
   constexpr size_t lds = Walk<BM, EPI, W8>::LDS;      // 256 / 192 / 160 / 128 rows: 160 / 145 / 137 / 160 KB; fp8 weights 128 / 113 / 105 / 112 KB
   static DeviceOnce attr_set;   // per instantiation
-  if (attr_set.first()) (void)hipFuncSetAttribute((const void*)gemm_walk_kernel<BM, EPI, W8>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  if (auto turn = attr_set.first()) (void)hipFuncSetAttribute((const void*)gemm_walk_kernel<BM, EPI, W8>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
   const unsigned grid = walk_grid((long)tiles_m * tiles_n, S);
   gemm_walk_kernel<BM, EPI, W8><<<dim3(grid, S), dim3(512), lds, st>>>(a.A, a.lda, a.W, a.bias, a.residual, a.ldr, a.C, a.ldc, a.M, a.N, a.K, tiles_m,
                                                                        tiles_n, a.partial, (nkt + S - 1) / S, raster_for(tiles_m), a.wscale);
@@ -1897,7 +1897,7 @@ static void launch_vit_rows(const GemmArgs& a, hipStream_t st) {
   constexpr size_t lds = Walk<BM, EPI == EPI_VIT_QKV ? EPI_VIT_QK : EPI>::LDS;
   static_assert(BM * 320 <= Walk<BM, EPI_VIT_QK>::SCRATCH, "the rotation's tables in the stages");
   static DeviceOnce attr_set;   // per instantiation
-  if (attr_set.first()) (void)hipFuncSetAttribute((const void*)gemm_vit_kernel<BM, EPI>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  if (auto turn = attr_set.first()) (void)hipFuncSetAttribute((const void*)gemm_vit_kernel<BM, EPI>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
   gemm_vit_kernel<BM, EPI><<<dim3(capped_grid((long)tiles_m * tiles_n)), dim3(512), lds, st>>>(a.A, a.lda, a.W, a.bias, a.C, a.ldc, a.M, a.N, a.K, tiles_m, tiles_n, a.vq,
                                                                                               raster_for(tiles_m));
 }
@@ -1933,7 +1933,7 @@ static void launch_vh(const GemmArgs& a, hipStream_t st) {
   const int tiles_m = vh_tiles(a.M, a.N, S).tiles_m, tiles_n = (a.N + 255) / 256;
   constexpr size_t lds = Walk<272, EPI>::LDS;      // stages, scratch, epilogue: 156,672 B
   static DeviceOnce attr_set;   // per instantiation
-  if (attr_set.first()) (void)hipFuncSetAttribute((const void*)gemm_walk_vh_kernel<EPI>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  if (auto turn = attr_set.first()) (void)hipFuncSetAttribute((const void*)gemm_walk_vh_kernel<EPI>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
   g_launch_counts[LC_GEMM_VH]++;
   const unsigned grid = walk_grid((long)tiles_m * tiles_n, S);
   gemm_walk_vh_kernel<EPI><<<dim3(grid, S), dim3(512), lds, st>>>(
@@ -1944,7 +1944,7 @@ static void launch_vh_small(const GemmArgs& a, hipStream_t st) {      // split-K
   const int nkt = a.K / 64, S = a.nsplit;
   constexpr size_t lds = (size_t)3 * (144 * 8 + 2048) * 16 + 1024;      // 3 x 51,200 B + the scratch
   static DeviceOnce attr_set;
-  if (attr_set.first()) (void)hipFuncSetAttribute((const void*)gemm_vh_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  if (auto turn = attr_set.first()) (void)hipFuncSetAttribute((const void*)gemm_vh_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
   g_launch_counts[LC_GEMM_VH]++;
   gemm_vh_kernel<<<dim3(capped_grid((long)tiles_m * tiles_n), S), dim3(512), lds, st>>>(a.A, a.lda, a.W, a.M, a.N, a.K, tiles_m, tiles_n, a.partial, (nkt + S - 1) / S,
                                                                                         raster_for(tiles_m));
@@ -2104,7 +2104,7 @@ template <int EPI, int MT, bool W8>
 static void launch_tall_rows(const GemmArgs& a, hipStream_t st) {
   constexpr size_t lds = Tall<MT, W8>::LDS;
   static DeviceOnce attr_set;   // per instantiation
-  if (attr_set.first()) (void)hipFuncSetAttribute((const void*)gemm_tall_kernel<EPI, MT, W8>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  if (auto turn = attr_set.first()) (void)hipFuncSetAttribute((const void*)gemm_tall_kernel<EPI, MT, W8>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
   gemm_tall_kernel<EPI, MT, W8><<<dim3((a.N + 159) / 160), dim3(512), lds, st>>>(a.A, a.lda, a.W, a.bias, a.residual, a.ldr, a.C, a.ldc, a.M, a.N, a.K, a.wscale);
 }
 template <int EPI, bool W8>

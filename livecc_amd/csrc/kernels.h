@@ -4,6 +4,7 @@
 #include <stdint.h>
 
 #include "../../include/livecc_amd.h"  // lcc_status codes
+#include "device_once.h"
 
 namespace lcc {
 
@@ -180,19 +181,6 @@ int sample_topk_topp(const void* logits, bool f32, int ld, int B, int V, uint32_
                      float repetition_penalty, int thr_token, int use_thr, float thr_value, int eos_token, int eos_token2,
                      int suppress_eos, int32_t* done, int32_t* out_tokens, int32_t* history, int hist_ld, int32_t* hist_col,
                      float* scores_out, float temperature, int top_k, float top_p, uint64_t seed, uint32_t* rng_ctr, hipStream_t st);
-// "first use on this device" latch for per-kernel attributes (160-KB dynamic LDS): hipFuncSetAttribute applies to the CURRENT device, so a
-// process that drives a second GPU must set it there too (the shipped deployment is one process per GPU).  Host only.
-struct DeviceOnce {
-  unsigned long long seen = 0;
-  bool first() {
-    int d = 0;
-    (void)hipGetDevice(&d);
-    const unsigned long long bit = 1ull << (d & 63);
-    if (seen & bit) return false;
-    seen |= bit;
-    return true;
-  }
-};
 // cur_tok / prev_tok (both or none): the token just consumed becomes the slot's previous token
 int read_slots(const int32_t* slots, int n, const int32_t* kv_len, const int32_t* pos, const int32_t* hist_col, const int32_t* history, int max_history, int take,
                const unsigned* err, int32_t* out, hipStream_t st);

@@ -703,7 +703,7 @@ template <bool CHUNK>
 static void attn_rows_launch(const Kv4Args& a, const Kv4Rows& rows, int n, const bf16_t* q, int n_q_heads, int nsplit, float* ws_o, float* ws_ml, bf16_t* out, hipStream_t st) {
   static DeviceOnce once;
   constexpr int part = 16 * 132 * 4;                                        // LDS of a wave's result
-  if (once.first()) (void)hipFuncSetAttribute((const void*)attn_rows_kv4_kernel<8, CHUNK>, hipFuncAttributeMaxDynamicSharedMemorySize, 8 * part);
+  if (auto turn = once.first()) (void)hipFuncSetAttribute((const void*)attn_rows_kv4_kernel<8, CHUNK>, hipFuncAttributeMaxDynamicSharedMemorySize, 8 * part);
   const dim3 grid(nsplit, a.n_kv_heads, n);
   if (nsplit == 1) attn_rows_kv4_kernel<8, CHUNK><<<grid, dim3(512), 8 * part, st>>>(a, rows, q, n_q_heads, nsplit, ws_o, ws_ml, out);
   else attn_rows_kv4_kernel<4, CHUNK><<<grid, dim3(256), 4 * part, st>>>(a, rows, q, n_q_heads, nsplit, ws_o, ws_ml, out);
@@ -1043,7 +1043,7 @@ int attn_prefill_kv4(const Kv4Args& a, const bf16_t* q, bf16_t* out, const int32
   if (nsplit > 1 && (ws_o == nullptr || ws_ml == nullptr)) return LCC_ERR_ARG;
   if (n_tiles == 0 || n_rows == 0) return 0;
   static DeviceOnce once;
-  if (once.first()) {
+  if (auto turn = once.first()) {
     (void)hipFuncSetAttribute((const void*)attn_chunk_kv4_kernel<8>, hipFuncAttributeMaxDynamicSharedMemorySize, KV4_LDS);
     (void)hipFuncSetAttribute((const void*)attn_chunk_kv4_kernel<4>, hipFuncAttributeMaxDynamicSharedMemorySize, KV4_LDS);
   }

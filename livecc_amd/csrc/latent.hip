@@ -488,7 +488,7 @@ static void latent_decode_go(const LatentDecodeArgs& a, hipStream_t st) {
   const int quads = (ht + groups - 1) / groups;
   const size_t lds = (size_t)NSTAGE * 8 * RT * 1024 + (size_t)quads * (16 * LATENT_PP * 2 + 256);
   static DeviceOnce once;   // per instantiation
-  if (once.first())
+  if (auto turn = once.first())
     (void)hipFuncSetAttribute((const void*)latent_attn_decode_kernel<RT, NSTAGE>, hipFuncAttributeMaxDynamicSharedMemorySize,
                               (int)((size_t)NSTAGE * 8 * RT * 1024 + (size_t)MAXQ * (16 * LATENT_PP * 2 + 256)));
   latent_attn_decode_kernel<RT, NSTAGE><<<dim3(a.nsplit, a.rows, groups), dim3(quads * 256), lds, st>>>(a);

@@ -451,7 +451,7 @@ template <int NT, bool OUT, bool SEGMENT>
 static void scan_go(const RecScanArgs& a, hipStream_t st) {
   constexpr size_t PK = NT * 64 + 8, lds = (64 * PK + 64 * 72) * 2 + 768 + (OUT ? 3 * 64 * PK * 2 : 0);
   static DeviceOnce once;   // per instantiation
-  if (once.first()) (void)hipFuncSetAttribute((const void*)rec_scan_kernel<NT, OUT, SEGMENT>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  if (auto turn = once.first()) (void)hipFuncSetAttribute((const void*)rec_scan_kernel<NT, OUT, SEGMENT>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
   rec_scan_kernel<NT, OUT, SEGMENT><<<dim3(a.n_seg, a.heads * (a.ep / 64)), dim3(256), lds, st>>>(a);
 }
 template <int NT>
