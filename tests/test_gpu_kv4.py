@@ -826,3 +826,47 @@ def test_no_route_loses_a_gradient(dev, through, monkeypatch):
         assert torch.equal(kv.buf, before), name
         with torch.no_grad():
             assert not call(**args).requires_grad
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("kv_heads", [1, 4])
+@pytest.mark.parametrize("rows", [1, 9, 61, 150, 333])
+def test_append_writes_its_own_bytes_and_no_others(dev, bits, kv_heads, rows):
+    """Every byte of every slot and layer against the layout: the bytes of the (slot, head, position) written, put back, leave the whole cache as it was; and each of them was written (two
+    fills).  Rows alone, and rows enough for V to go by windows; runs that begin and end within octets, rows of no stream and of positions outside between them."""
+    from livecc_amd import ops
+    n, lmax, layers, layer, heads = 4, 192, 3, 1, 3
+    at, S = [], rows
+    for i in range(rows):                                        # slots 2 and 0, slot 1 stays; 13 .. upwards and 190 .. downwards
+        at.append((2, 13 + i // 2) if i % 2 == 0 and rows < 100 else (0, 190 - i) if rows < 100 else (2, 5 + i) if i < 180 else (0, i - 177))
+        if i % 23 == 11:
+            at[-1] = ((-1, 3), (2, lmax), (n, 7), (0, -1))[i // 23 % 4]
+    stream, pos = (i32([a[z] for a in at], dev) for z in range(2))
+    live = [(s, p) for s, p in at if 0 <= s < n and 0 <= p < lmax]
+    assert len(set(live)) == len(live)
+    s, p = (torch.tensor([a[z] for a in live]) for z in range(2))
+    h = torch.arange(kv_heads)[None, :, None]
+    if bits == 16:                                               # [layer][K [head][position][128] | V [head][position / 32][128][position % 32]], bf16
+        c, kv_layer = torch.arange(128), 2 * kv_heads * lmax * 128
+        k = (h * lmax + p[:, None, None]) * 128 + c
+        v = ((kv_heads + h) * lmax + p[:, None, None] // 32 * 32) * 128 + c * 32 + p[:, None, None] % 32
+        own = [(layer * kv_layer + torch.cat((k, v), -1))[..., None] * 2 + torch.arange(2)]
+    else:                                                        # [layer][K codes | V codes | K scales | V scales], bytes
+        q, g, e = p[:, None, None], p[:, None, None] % 32 // 8, p[:, None, None] % 8
+        it, t, base = torch.arange(64), torch.arange(4), layer * kv_heads * lmax * 136
+        own = [base + (h * lmax + q) * 64 + it, base + (kv_heads + h) * lmax * 64 + q // 32 * 2048 + g * 512 + it * 8 + e,
+               base + kv_heads * lmax * 128 + (h * lmax + q) * 4 + t, base + kv_heads * lmax * 132 + h * lmax * 4 + q // 32 * 128 + g * 32 + t * 8 + e]
+    own = torch.cat([x.reshape(len(live), -1) for x in own], 1)
+    assert own.shape[1] == kv_heads * (512 if bits == 16 else 136)
+    qkv, (cos, sin) = rand((S, (heads + 2 * kv_heads) * 128), dev, rows), tables([a[1] for a in at], dev)
+    w, written = rand((128,), dev, 2), []
+    for fill in (0x3B, 0xC4):
+        kv = (ops.Kv4Arena if bits == 4 else ops.KvArena)(n, layers, kv_heads, lmax, dev)
+        kv.buf.view(torch.uint8).fill_(fill)
+        ops.qk_norm_rope_kv_append(qkv, cos, sin, stream, pos, kv, layer, heads, q_norm=w, k_norm=w)
+        held = kv.buf.view(torch.uint8).cpu()
+        assert held.shape[1] > int(own.max())
+        written.append(held[s[:, None], own].clone())
+        held[s[:, None], own] = fill
+        assert bool((held == fill).all()), f"{int((held != fill).sum())} bytes of others"
+    assert torch.equal(*written)
