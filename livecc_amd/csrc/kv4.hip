@@ -62,8 +62,8 @@ LCC_DEVICE u32x4 fp4_word(unsigned w, unsigned scale) { return (u32x4){fp4_pair<
 
 // ------------------------------------------------------------------------------------------------------------------------------
 // Norm, rotation, append: every head row of a token is read once and written once (queries as bf16, keys and values into the cache).
-// Bound: up to some 400 rows the trips to a row, its place and the cache (2.7 us for a row of 28 / 4 heads, 4.5 us for 386); 9,048 rows 36.8 us for 169 MB, 4,076 rows of 64 / 8 heads into
-// 4 bits 32 us for 155 MB, 4.6-4.8 TB/s, where a copy of the same bytes takes 34 and 31: the vector work (the norm and eight roundings a pair, some 350 instructions a wave, 25 us by
+// Bound: up to some 400 rows the trips to a row, its place and the cache (2.7 us for a row of 28 / 4 heads, 4.6 us for 386; into 4 bits 4.5 us for eight rows of 12 / 2, whose arena's address is
+// loaded behind the norm); 9,048 rows 33 to 36 us for 169 MB, 4,076 rows of 64 / 8 heads into 4 bits 31 to 33 us for 155 MB, 4.7-5.1 TB/s, where a copy of the same bytes takes 34 and 31: the vector work (the norm and eight roundings a pair, some 350 instructions a wave, 25 us by
 // themselves) hides behind the memory as long as all loads of a lane are in flight before the first wait (one after the other: 3 us more) and V is stored by whole octets.  Blocks that stay
 // and fetch their next item ahead were no faster, nor four heads a lane group behind one load of the tables; sums in 32 bits would save nothing.
 // ------------------------------------------------------------------------------------------------------------------------------
@@ -155,9 +155,13 @@ LCC_DEVICE void head_norm(float (&x1)[8], float (&x2)[8], const u32x4& w1, const
   }
 }
 
-// From so many rows on V goes by windows (us, without and with; 28 / 4 heads unless said).  A chunk of 128 rows 4.4 / 3.8 (4 bits 4.5 / 4.3), of 386 5.8 / 4.5 (5.5 / 4.9), of 1,131 10.7 / 7.0
-// (8.4 / 7.0); 600 tokens of as many streams, no octet among them, 8.7 / 8.5 (6.3 / 6.6).  It costs most with 64 / 8 heads in 4 bits: 386 rows 6.3 / 6.7, 600 tokens 7.8 / 9.7.  Below, one
-// wave's row is as quick: 64 rows 4.2 / 3.7 (4.5 / 4.2), and batches of single tokens are of that size.
+// From so many rows on V goes by windows.  Without / with them, us a call:
+//   chunks        64 rows       128           386           1,131           single tokens of as many streams (no octet among them)   64            128           600
+//   28 / 4, bf16  3.8 / 3.4     4.0 / 3.6     5.4 / 4.2     10.9 / 7.2                                                               3.8 / 5.1     4.3 / 5.6     9.0 / 9.3
+//   28 / 4, 4 b.  4.1 / 4.0     4.1 / 4.1     5.0 / 4.6     8.8 / 7.3                                                                4.1 / 4.8     4.1 / 4.9     6.0 / 6.7
+//   64 / 8, bf16  3.7 / 3.7     4.5 / 3.9     8.2 / 6.3     15.7 / 11.8                                                              3.8 / 5.6     5.2 / 6.7     13.8 / 14.2
+//   64 / 8, 4 b.  3.4 / 4.1     3.9 / 4.3     6.1 / 6.6     11.7 / 11.7                                                              3.3 / 4.9     3.9 / 5.5     8.4 / 10.0
+// Below 128 rows a chunk gains 0.4 us at most and a batch of single tokens loses 0.7 to 1.8; decode batches are of that size, larger calls are mostly chunks.
 constexpr int KV4_WINDOW_ROWS = 128;
 // Where a row's keys and values go: its slot and position, slot -1 for a row of no stream or no position.
 LCC_DEVICE void row_place(const QkNormArgs& a, int s, int& slot, int& pos) {
@@ -404,8 +408,8 @@ int qk_norm_rope_append(const QkNormArgs& a, bool kv4, hipStream_t st) {
 
 // ------------------------------------------------------------------------------------------------------------------------------
 // Read-back: row s = (slot, position) -> its keys and values [heads][128] in bf16; a row of no stream or position: zeros.  Eight lanes a (row, head), 16 channels
-// each; rows run innermost, so that the bytes of V a wave gathers lie side by side where rows are neighbours (4,076 rows of 8 heads 8.1 -> 6.8 us; 21 MB).  Bound: two
-// trips, to the row's place and to its bytes.
+// each; rows run innermost, so that the bytes of V a wave gathers lie side by side where rows are neighbours (heads innermost: 1.3 us more).  4,076 rows of 8 heads 6.6 to 7.4 us for 21 MB,
+// 3 TB/s.  Bound: a lane waits for its row's place, and behind it for eight single bytes of V, 32 bytes apart.
 // ------------------------------------------------------------------------------------------------------------------------------
 __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4Args a, const int32_t* __restrict__ tok_stream, const int32_t* __restrict__ tok_pos,
                                                        bf16_t* __restrict__ k_out, bf16_t* __restrict__ v_out, int rows) {
@@ -451,8 +455,8 @@ int kv4_read(const Kv4Args& a, const int32_t* tok_stream, const int32_t* tok_pos
 // 8 g .. 8 g + 7, which are the slots of its P operand: O^T += V^T P^T takes the probabilities from the softmax' registers and V's bytes as they lie.
 // The loads of a wave's next block go into the registers that the products have just left, K's first, so that either is waited for by a count while the other is in flight; 126
 // registers, 16 waves a unit (a second set of them: spills at that occupancy, and no gain at half of it).
-// Bound: 64 rows of 2,200 to 6,000 keys (28 / 4 heads) 32 us for 139 MB, 4.3 TB/s where a large copy moves 4.95 both ways together; the arithmetic alone takes 25 us.  One row of
-// 32,768 keys (64 / 8 heads, 64 splits) 10 us for 36 MB, of which some 4 are the launch and the first trip.
+// Bound: 64 rows of 2,200 to 6,000 keys (28 / 4 heads) 32 us for 139 MB, 4.3 TB/s where a read stream reaches 6.0 (38 us where other data has passed the 256 MB cache in between); the
+// arithmetic alone takes 25 us.  One row of 32,768 keys (64 / 8 heads, 32 splits) 9.8 us for 36 MB, of which some 4 are the launch and the first trip.
 // The same kernel takes tiles of a few rows of a chunk (CHUNK): its columns are then (row, head) pairs.
 // ------------------------------------------------------------------------------------------------------------------------------
 // Scores are sums of products q k; a weight is 2^(KV4_SCALE (score - m)), the difference formed before it is scaled: m scaled by itself is off by half a step, which is more than 2^7 powers of
@@ -631,8 +635,8 @@ __global__ __launch_bounds__(NW * 64, 4) void attn_rows_kv4_kernel(Kv4Args a, Kv
 }
 
 // Joins the key splits of a (row, head): sums weighted by their m's distance from the highest, one rounding.  A half-wave reads a split's 128 channels at a time; W waves share a (row, head).
-// blockIdx.y: a tile, or (tiles null) a row.  All loads of a (row, head) are in flight before the first weight is known; a trip's time otherwise: 64 splits of 64 heads 3.6 us,
-// of 17 rows x 28 4.3 us (15.8 MB), five of 386 rows 7.6 us (28 MB, 3.7 TB/s).  In one wave (W = 1) to 8 splits, in four beyond: those have more to load than registers.
+// blockIdx.y: a tile, or (tiles null) a row.  All loads of a (row, head) are in flight before the first weight is known; a trip's time otherwise: 32 splits of 64 heads 3.5 us,
+// 64 of 17 rows x 28 4.3 us (15.8 MB), five of 386 rows x 28 7.7 us (28 MB, 3.7 TB/s).  In one wave (W = 1) to 8 splits, in four beyond: those have more to load than registers.
 template <int W>
 __global__ __launch_bounds__(256) void kv4_combine_kernel(const float* __restrict__ ws_o, const float* __restrict__ ws_ml, bf16_t* __restrict__ out,
                                                           const int32_t* __restrict__ tile_q0, const int32_t* __restrict__ tile_nq, int tile_rows, int n_rows, int n_q_heads,
@@ -689,6 +693,8 @@ static void kv4_combine(const float* ws_o, const float* ws_ml, bf16_t* out, cons
 //   More: eight, from 96 key blocks on, where the blocks leave a fifth of the units or more idle in their last round: 40 rows of 2,400 keys 1 / 2 / 8 splits 13.6 / 16.5 / 16.6, of 6,144
 //   34.0 / 36.2 / 30.1; 24 rows of 2,400 13.0 / 12.7 / 12.7, of 6,144 26.2 / 20.4 / 18.0; 48 of 16,000 88.6 / 90.6 / 74.9; 80 of 6,000 65.4 / 59.7 / 53.7.  Where the round is full, from 320 on:
 //   64 rows of 6,144 keys 1 / 6 splits 45.2 / 44.9, 56 rows 41.1 / 40.3, 128 rows of 6,000 1 / 8 splits 83.8 / 84.1, of 12,000 161.3 / 160.0, with lengths over two thirds 128.8 / 124.9.
+// One count serves all rows of a launch, so a long row among short ones is split as if all were long: 32,000 keys alone 9.8 us (64 splits), beside 7 rows of 500 23.8 (eight; 32 splits would
+// take 12.9), beside 63 26.6 (16: 22.8); 9,000 keys alone 7.9, beside 63 rows of 500 35.9 (unsplit; eight: 15.4).
 int kv4_decode_splits(const int32_t* n_keys, int n, int n_kv_heads) {
   long most = 1;
   for (int i = 0; i < n; ++i) most = n_keys[i] > most ? n_keys[i] : most;
@@ -727,8 +733,9 @@ int attn_decode_kv4(const Kv4Args& a, const bf16_t* q, const int32_t* slots, con
 // O^T += V^T P^T on 32x32x16, K's rows read in the order (bits 2 and 3 swapped) that leaves a lane the scores of the keys its P operand wants.
 // Conversion once a block and stage is what LDS is for: 8 KB of codes become 32 KB that all waves read, in images whose 16-byte chunks are permuted so that neither the reads (16 lanes at
 // a time) nor the writes (8) meet in a bank (no conflicts counted).
-// Bound: eight chunks of ~340 rows on ~5,000 keys 243 us, 0.86 PFLOP/s where a large matrix product reaches 1.20: of a wave's 64-key stage 1,024 clocks are matrix instructions and some 950
-// vector ones (conversion, softmax), and the two waves of a SIMD overlap them by little (matrix units busy half of the time).  Other orders of the stage, pinned or with
+// Eight chunks of ~340 rows on ~5,000 keys 242 to 252 us, 0.83-0.87 PFLOP/s where a large matrix product reaches 1.4 (the bf16 cache's attention takes 262 for them): of a wave's 64-key stage
+// 1,024 clocks are matrix instructions and some 950 vector ones (conversion, softmax), and the counters show that the two waves of a SIMD overlap them by little (matrix units busy half of the
+// time).  Other orders of the stage, pinned or with
 // priorities, were no faster (159 -> 170 us for 386 rows unsplit); products in the 4-bit type itself, with queries in parts of 8 bits, sum to 2^-13.5 only and were not taken.
 // Few rows: 17 rows of 28 / 4 heads on 26,800 keys 21 us, a third of it the 64 splits' partials (15.8 MB).
 // ------------------------------------------------------------------------------------------------------------------------------
