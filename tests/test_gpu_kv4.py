@@ -870,3 +870,52 @@ def test_append_writes_its_own_bytes_and_no_others(dev, bits, kv_heads, rows):
         held[s[:, None], own] = fill
         assert bool((held == fill).all()), f"{int((held != fill).sum())} bytes of others"
     assert torch.equal(*written)
+
+
+@pytest.mark.parametrize("through", ["torch", "ctypes"])
+@pytest.mark.parametrize("columns", [16, 128, 256])
+@pytest.mark.parametrize("nsplit", [1, 2])
+def test_chunk_rows_below_position_zero_see_nothing(dev, through, columns, nsplit):
+    """A tile that begins below zero: its rows there are zeros, whatever the first keys hold (NaN among them), the others see keys 0 .. p."""
+    heads, kv_heads, lmax, height = 14, 2, 96, columns * 2 // 14
+    k, v = rand((2, kv_heads, lmax, 128), dev, 1), rand((2, kv_heads, lmax, 128), dev, 2)
+    k[1, :, 0, 5] = v[1, :, 0, :] = math.nan
+    kv = filled(dev, k, v)
+    runs = [(0, 12, -5), (1, 12, -5), (0, 3, -3), (1, 2, -2 ** 31), (0, 2, -1)]
+    tiles, at = [], []
+    for slot, n, pos in runs:
+        tiles += [(slot, len(at) + o, min(height, n - o), pos + o) for o in range(0, n, height)]
+        at += [(slot, pos + r) for r in range(n)]
+    q = rand((len(at), heads * 128), dev, 3)
+    got = by_tiles(through, q, kv, tiles, heads, height, nsplit)
+    for i, (slot, p) in enumerate(at):
+        if p < 0:
+            assert not got[i].any(), (i, p)
+        elif slot == 1:
+            assert bool(torch.isnan(got[i]).all()), (i, p)
+        else:
+            want, tol = U.attention(q[i:i + 1].cpu().view(1, heads, 128), *values(kv, slot), [p])
+            U.assert_within(got[i], want[0].flatten(), tol[0].flatten(), f"row {i}, position {p}")
+
+
+@pytest.mark.parametrize("nsplit", [1, 2])
+def test_as_many_rows_and_tiles_as_a_launch_takes(dev, nsplit):
+    """65,535 rows of a decode step and 65,535 tiles of a chunk, each as alone; one more is refused"""
+    from livecc_amd import ops
+    heads, kv_heads, L, most = 2, 1, 64, 65535
+    kv = filled(dev, rand((3, kv_heads, L, 128), dev, 1), rand((3, kv_heads, L, 128), dev, 2))
+    q = rand((most + 1, heads * 128), dev, 3)
+    slots, lens = torch.arange(most + 1, dtype=torch.int32, device=dev) % 4 - 1, i32([63, 40, 0], dev)
+    got = ops.attn_decode4(q[:most], kv, 0, slots[:most], lens, heads, nsplit)
+    for i in (0, 1, 2, 3, 32768, 65533, 65534):
+        assert torch.equal(got[i:i + 1], ops.attn_decode4(q[i:i + 1], kv, 0, slots[i:i + 1], lens, heads, nsplit)), i
+    assert not got[slots[:most] < 0].any()
+    plan = ops.kv4_prefill_plan([(r % 3, 1, r % 61) for r in range(most)], heads, kv_heads, dev, nsplit, 4)
+    got = ops.attn_prefill4(q[:most], kv, 0, plan, heads)
+    for i in (0, 1, 60, 32768, 65534):
+        one = ops.kv4_prefill_plan([(i % 3, 1, i % 61)], heads, kv_heads, dev, nsplit, 4)
+        assert torch.equal(got[i:i + 1], ops.attn_prefill4(q[i:i + 1], kv, 0, one, heads)), i
+    with pytest.raises(RuntimeError):
+        ops.attn_decode4(q, kv, 0, slots, lens, heads, nsplit)
+    with pytest.raises(RuntimeError):
+        ops.attn_prefill4(q, kv, 0, ops.kv4_prefill_plan([(0, 1, 0)] * (most + 1), heads, kv_heads, dev, nsplit, 4), heads)
